@@ -33,6 +33,7 @@ enum {
   R4Q_ERR_CAPACITY = -3,   /* workspace / scratch too small */
   R4Q_ERR_CUDA = -4,       /* a CUDA runtime call failed */
   R4Q_ERR_TIMEOUT = -5,    /* a bounded device-side wait gave up */
+  R4Q_ERR_PAGE = -6,       /* a kernel met a page id, position or row outside the paged cache */
 };
 
 /* Activation prologue applied inside the GEMV before the dot products. */
@@ -226,6 +227,92 @@ int r4q_dequant_int8(const void* w, const void* s, void* out, int N, int K, void
 int r4q_kv_write_rows(const void* k, const void* v, long ld, void* k_cache, void* v_cache, int M, int Hk, int D,
                       int max_seq, int start_pos, int batch_row, const float* k_scale, const float* v_scale,
                       void* stream);
+
+/* ------------------------------------------------------------ paged cache --- */
+/* No counterpart in the reference, whose cache is one max_seq row per request.
+ * One layer's FP8 K and V in pages of `page` positions (a multiple of 16):
+ * uint8 [n_pages][Hk][page][128] each, pages k_stride / v_stride bytes apart
+ * (multiples of 16; 0: contiguous).  Position p of sequence b is row p % page
+ * of page table[b * ld_table + p / page]; sequences may share pages.  The
+ * scales, one per kv head, belong to the pool (stored byte = enc(x / scale)),
+ * so that a shared page reads alike from every sequence. */
+typedef struct r4q_paged_cache {
+  void *k_pages, *v_pages;
+  long k_stride, v_stride;
+  int n_pages, page, Hk;
+  const int* table;            /* device int32 [seqs][ld_table], max_blocks entries used per row */
+  long ld_table;
+  int seqs, max_blocks;
+  const float *k_scale, *v_scale;   /* fp32 [Hk] or NULL */
+} r4q_paged_cache;
+
+enum { R4Q_KV_FULL_RANGE = 8 };
+/* M new tokens into the pages: token m goes to position pos[m] (int64, device)
+ * of sequence rows[m] (int32, device; NULL: sequence m).  k, v: fp16 [M] rows
+ * ldk / ldv apart with Hk heads of 128; q (NULL or H = 0: none): H heads, ldq.
+ * Flags R4Q_HEAD_NORM / R4Q_HEAD_ROPE apply the per-head RMSNorm and the
+ * half-split rotation (row pos[m] of the tables, fp16 [tab_rows][tab_stride])
+ * to q and k first, in fp32 with one rounding, as r4q_head_norm_rope does;
+ * q_out (ldqo) and k_out (ldko; NULL skips) receive them and may alias q, k.
+ * The stored bytes are those of r4q_head_norm_rope's KV write.  That codec
+ * stores every |x / scale| from 248 on as 448; with R4Q_KV_FULL_RANGE 256 .. 448
+ * are stored as E4M3 has them (all readers decode both), for scales that bring
+ * the largest values near 448.
+ * A token with pos[m] < 0 is padding: nothing of it is read or written.  A row,
+ * position, page or table row out of range writes nothing and is reported by
+ * r4q_paged_status.  Two tokens of one call must not name one position.
+ * 16-byte aligned pointers, row strides in multiples of 8 elements. */
+int r4q_paged_kv_write(const void* q, long ldq, const void* k, long ldk, const void* v, long ldv,
+                       const void* q_norm_w, const void* k_norm_w, const void* cos_tab, const void* sin_tab,
+                       long tab_stride, long tab_rows, void* q_out, long ldqo, void* k_out, long ldko,
+                       const r4q_paged_cache* cache, const int* rows, const long long* pos, int M, int H,
+                       float eps, int flags, void* stream);
+
+/* o[b, h] = softmax(q[b,h]·K^T / sqrt(128)) V over positions [0, seq_lens[b])
+ * of sequence b, as r4q_flash_decode over a contiguous cache (fp32 softmax and
+ * sums, fp16 out, R4Q_ATTN_FWHT, zeros for an empty sequence).  B <= cache->seqs
+ * rows; seq_lens int64 [B], device; any H that is a multiple of Hk.  A page id
+ * outside the pool reads as zeros, a length beyond max_blocks * page is cut;
+ * both are reported by r4q_paged_status.  Bytes of a page behind the sequence
+ * may hold anything.  workspace (16-byte aligned, of the size that
+ * r4q_paged_flash_decode_workspace_bytes gives; may be 0, then NULL) needs no
+ * initialisation and keeps nothing between calls; calls that may run at once
+ * need one each. */
+size_t r4q_paged_flash_decode_workspace_bytes(int B, int H, int Hk, int page, int max_blocks);
+int r4q_paged_flash_decode(const void* q, long ldq, const r4q_paged_cache* cache, const long long* seq_lens, void* o,
+                           long ldo, int B, int H, int flags, void* workspace, size_t ws_bytes, void* stream);
+
+/* R4Q_ERR_PAGE / R4Q_ERR_TIMEOUT if a paged kernel of the current device met an
+ * id out of range / gave up a wait since the last clear, else R4Q_OK.
+ * Synchronises the device. */
+int r4q_paged_status(int clear);
+
+/* pool[l][dst[i]] = pool[l][src[i]] for every i < n and every l < outer: pages of
+ * page_bytes, page_stride apart, in `outer` pools (layers, K and V)
+ * outer_stride bytes apart.  src and dst are HOST arrays, read before the call
+ * returns; a page may be copied to several places, but is written once at most
+ * and not both read and written.  Sizes, strides and pool in multiples of 16. */
+int r4q_kv_copy_pages(void* pool, long outer, long outer_stride, long page_stride, long page_bytes, int n_pages,
+                      const int* src, const int* dst, int n, void* stream);
+/* table[r[i] * ld + c[i]] = v[i] (device int32 [rows][ld]); r, c, v are HOST arrays of
+ * n, read before the call returns; no cell twice. */
+int r4q_kv_table_set(int* table, long ld, int rows, int cols, const int* r, const int* c, const int* v, int n,
+                     void* stream);
+
+/* -------------------------------------------------------- token likelihoods --- */
+enum { R4Q_T_F16 = 0, R4Q_T_BF16 = 1, R4Q_T_F32 = 2 };
+/* Of every row of logits [M, V] (R4Q_T_*, ld elements apart) and its token:
+ * logprob = x_t - lse, rank = 1 + the ids that precede t by (value, lowest id
+ * first), entropy = lse - sum p x in nats, and the k <= 32 (and <= V) most
+ * likely ids in that order with their log probabilities, [M, k].  Sums in fp32
+ * over one pass.  tokens int64 [M] (NULL: only entropy and top); an id outside
+ * [0, V) gets logprob NaN and rank 0.  A row with NaN or +inf, or with nothing
+ * above -inf, has no distribution: its log probabilities and entropy are NaN
+ * (NaN counts as the lowest value in the order).  Outputs may be NULL.
+ * The reference returns no likelihoods (api_server.py:58-150). */
+int r4q_token_logprobs(const void* logits, int type, long ld, const long long* tokens, int M, int V, int k,
+                       float* logprob, long long* rank, float* entropy, long long* top_ids, float* top_logprobs,
+                       void* stream);
 
 /* ------------------------------------------------- mixture-of-experts FFN --- */
 /* No counterpart in the reference (its engine is dense); benchmark config 4.

@@ -1,0 +1,323 @@
+// Paged FP8 KV cache: new tokens into pages (with the per-head RMSNorm + RoPE
+// of q and k), page copies over all layers, block-table updates, and the
+// status word of the paged kernels.
+#include <cstring>
+#include <vector>
+
+#include "paged.cuh"
+#include "r4q_common.cuh"
+
+namespace r4q {
+namespace {
+
+__device__ int g_write_status;
+
+// ---------------------------------------------------------------- KV write
+// A warp takes kHeads consecutive heads of one token (H of q, Hk of k, Hk of v),
+// so that the token's position, page and rotation row are looked up once and
+// kHeads loads are in flight together.  Lane l holds elements 2l, 2l + 1 and
+// 64 + 2l, 65 + 2l: 4-byte accesses that a warp makes contiguous, and the RoPE
+// partners i, i + 64 in one lane.  Norm and rotation are those of head_kernel
+// (r4q_head_norm_rope) to the bit, so a paged cache holds the bytes that the
+// contiguous one would: the sum of squares runs over elements r, r + 32,
+// r + 64, r + 96 first and then pairwise over r, which here takes the values
+// of lane l ^ 16 and a butterfly over two partial sums per lane.
+constexpr int kHeads = 4;
+struct WriteArgs {
+  const __half *q, *k, *v;
+  long ldq, ldk, ldv;
+  const __half *qw, *kw, *cos_tab, *sin_tab;
+  long tab_stride, tab_rows;
+  __half *q_out, *k_out;
+  long ldqo, ldko;
+  PagedView c;
+  const int* rows;
+  const long long* pos;
+  int M, H, groups;                // groups of kHeads heads per token
+  float eps;
+  int flags;
+};
+
+// rsqrt(mean(x^2) + eps) of the head that the warp holds as (2l, 2l+1, 64+2l, 65+2l)
+__device__ __forceinline__ float head_rrms(const float (&x)[4], float eps, int lane) {
+  float s[2];
+#pragma unroll
+  for (int a = 0; a < 2; ++a) {
+    const float y0 = __shfl_xor_sync(0xffffffffu, x[a], 16), y1 = __shfl_xor_sync(0xffffffffu, x[2 + a], 16);
+    const bool low = lane < 16;
+    const float v0 = low ? x[a] : y0, v1 = low ? y0 : x[a], v2 = low ? x[2 + a] : y1, v3 = low ? y1 : x[2 + a];
+    float ss = 0.0f;
+    ss += v0 * v0;
+    ss += v1 * v1;
+    ss += v2 * v2;
+    ss += v3 * v3;
+    s[a] = ss;
+  }
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) {
+    s[0] += __shfl_xor_sync(0xffffffffu, s[0], d);
+    s[1] += __shfl_xor_sync(0xffffffffu, s[1], d);
+  }
+  return rsqrtf((s[0] + s[1]) / (float)kHeadDim + eps);
+}
+// The cache codec (fp8_encode), or with `full` the same rounding without its
+// saturation of the whole top binade: 256 .. 448 are kept as E4M3 has them.
+__device__ __forceinline__ uint32_t encode(float x, bool full) {
+  const uint32_t r = fp8_encode(x);
+  if (!full || (r & 0x7Fu) != 0x7Eu) return r;
+  const uint32_t f = __float_as_uint(fminf(fabsf(x), 448.0f));      // 248 .. 448, NaN as 448
+  const uint32_t m = (f >> 20) + ((f >> 19) & 1u);                  // exponent and 3 bits, ties away from zero
+  return (r & 0x80u) | (m - (120u << 3));
+}
+__device__ __forceinline__ uint32_t encode2(float a, float b, const float* scale, int kh, bool full) {
+  const float s = scale ? scale[kh] : 1.0f;
+  return encode(scale ? a / s : a, full) | (encode(scale ? b / s : b, full) << 8);
+}
+
+__global__ void __launch_bounds__(256) paged_write_kernel(const WriteArgs a) {
+  const int lane = threadIdx.x & 31;
+  const long w = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const long m = w / a.groups;
+  if (m >= a.M) return;
+  const int h0 = (int)(w - m * a.groups) * kHeads, nh = a.H + 2 * a.c.Hk;
+  const long long pos = a.pos[m];
+  if (pos < 0) return;
+  const long row = a.rows ? a.rows[m] : m;
+  bool ok = row >= 0 && row < a.c.seqs && pos < (long long)a.c.max_blocks * a.c.page;
+  if (ok && (a.flags & R4Q_HEAD_ROPE)) ok = pos < a.tab_rows;
+  int pg = 0;
+  if (ok) {
+    pg = a.c.table[row * a.c.ld_table + (int)pos / a.c.page];
+    ok = pg >= 0 && pg < a.c.n_pages;
+  }
+  if (!ok) {
+    if (lane == 0) atomicOr(&g_write_status, kPagedBadPage);
+    return;
+  }
+  float x[kHeads][4];
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const int h = h0 + i;
+    if (h >= nh) break;
+    const __half* src = h < a.H               ? a.q + m * a.ldq + (long)h * kHeadDim
+                        : h < a.H + a.c.Hk    ? a.k + m * a.ldk + (long)(h - a.H) * kHeadDim
+                                              : a.v + m * a.ldv + (long)(h - a.H - a.c.Hk) * kHeadDim;
+    const uint32_t* s32 = reinterpret_cast<const uint32_t*>(src);
+    const float2 lo = __half22float2(u32_as_h2(s32[lane])), hi = __half22float2(u32_as_h2(s32[lane + 32]));
+    x[i][0] = lo.x; x[i][1] = lo.y; x[i][2] = hi.x; x[i][3] = hi.y;
+  }
+  float2 c{1.f, 1.f}, s{0.f, 0.f};
+  if (a.flags & R4Q_HEAD_ROPE) {
+    c = __half22float2(u32_as_h2(reinterpret_cast<const uint32_t*>(a.cos_tab + pos * a.tab_stride)[lane]));
+    s = __half22float2(u32_as_h2(reinterpret_cast<const uint32_t*>(a.sin_tab + pos * a.tab_stride)[lane]));
+  }
+  const long in_page = (long)((int)pos % a.c.page) * kHeadDim;
+  const bool full = a.flags & R4Q_KV_FULL_RANGE;
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const int h = h0 + i;
+    if (h >= nh) break;
+    const bool is_q = h < a.H, is_v = h >= a.H + a.c.Hk;
+    const int kh = is_q ? 0 : is_v ? h - a.H - a.c.Hk : h - a.H;
+    float(&v)[4] = x[i];
+    if (!is_v) {
+      if (a.flags & R4Q_HEAD_NORM) {
+        const float rrms = head_rrms(v, a.eps, lane);
+        const uint32_t* w32 = reinterpret_cast<const uint32_t*>(is_q ? a.qw : a.kw);
+        const float2 lo = __half22float2(u32_as_h2(w32[lane])), hi = __half22float2(u32_as_h2(w32[lane + 32]));
+        v[0] = v[0] * rrms * lo.x;
+        v[1] = v[1] * rrms * lo.y;
+        v[2] = v[2] * rrms * hi.x;
+        v[3] = v[3] * rrms * hi.y;
+      }
+      if (a.flags & R4Q_HEAD_ROPE) {
+        const float e0 = v[0], o0 = v[2], e1 = v[1], o1 = v[3];
+        v[0] = e0 * c.x - o0 * s.x;
+        v[2] = o0 * c.x + e0 * s.x;
+        v[1] = e1 * c.y - o1 * s.y;
+        v[3] = o1 * c.y + e1 * s.y;
+      }
+    }
+    __half* out = is_q ? a.q_out + m * a.ldqo + (long)h * kHeadDim
+                       : !is_v && a.k_out ? a.k_out + m * a.ldko + (long)kh * kHeadDim : nullptr;
+    if (out) {
+      uint32_t* o32 = reinterpret_cast<uint32_t*>(out);
+      o32[lane] = h2_as_u32(__floats2half2_rn(v[0], v[1]));
+      o32[lane + 32] = h2_as_u32(__floats2half2_rn(v[2], v[3]));
+    }
+    if (is_q) continue;
+    uint8_t* dst = (is_v ? a.c.v + pg * a.c.v_stride : a.c.k + pg * a.c.k_stride) +
+                   (long)kh * a.c.page * kHeadDim + in_page;
+    const float* scale = is_v ? a.c.v_scale : a.c.k_scale;
+    reinterpret_cast<uint16_t*>(dst)[lane] = (uint16_t)encode2(v[0], v[1], scale, kh, full);
+    reinterpret_cast<uint16_t*>(dst)[lane + 32] = (uint16_t)encode2(v[2], v[3], scale, kh, full);
+  }
+}
+
+// ------------------------------------------------------------- page copies
+constexpr int kMaxMoves = 448;          // (src, dst) pairs in one launch's parameters (3.5 KB)
+struct Moves {
+  int src[kMaxMoves], dst[kMaxMoves];
+};
+
+__global__ void __launch_bounds__(256)
+    copy_pages_kernel(uint8_t* pool, long outer_stride, long page_stride, long page_bytes,
+                      const __grid_constant__ Moves mv) {
+  const int i = blockIdx.x;
+  uint8_t* base = pool + (long)blockIdx.y * outer_stride;
+  const uint4* s = reinterpret_cast<const uint4*>(base + (long)mv.src[i] * page_stride);
+  uint4* d = reinterpret_cast<uint4*>(base + (long)mv.dst[i] * page_stride);
+  for (long j = threadIdx.x; j < page_bytes / 16; j += blockDim.x) d[j] = s[j];
+}
+
+constexpr int kMaxCells = 320;
+struct Cells {
+  int r[kMaxCells], c[kMaxCells], v[kMaxCells];
+};
+__global__ void table_set_kernel(int* table, long ld, int n, const __grid_constant__ Cells cells) {
+  for (int i = threadIdx.x; i < n; i += blockDim.x) table[cells.r[i] * ld + cells.c[i]] = cells.v[i];
+}
+
+}  // namespace
+
+int paged_view(const char* what, const r4q_paged_cache* c, PagedView* out) {
+  if (!c || !c->k_pages || !c->v_pages || !c->table) return set_error(R4Q_ERR_ARG, "%s: null cache pointer", what);
+  if (c->page < 16 || c->page % 16 || c->page > 4096)
+    return set_error(R4Q_ERR_ARG, "%s: page of %d positions (a multiple of 16, at most 4096)", what, c->page);
+  if (c->n_pages < 1 || c->Hk < 1 || c->Hk > 65535 || c->seqs < 1 || c->max_blocks < 1 || c->ld_table < c->max_blocks)
+    return set_error(R4Q_ERR_ARG, "%s: bad cache (pages %d, kv heads %d, table %d x %d)", what, c->n_pages, c->Hk,
+                     c->seqs, c->max_blocks);
+  if ((long)c->Hk * c->page > (1L << 24) || (long)c->max_blocks * c->page > (1L << 30))
+    return set_error(R4Q_ERR_ARG, "%s: Hk * page above 2^24 or max_blocks * page above 2^30", what);
+  const long bytes = (long)c->Hk * c->page * kHeadDim;
+  const long ks = c->k_stride ? c->k_stride : bytes, vs = c->v_stride ? c->v_stride : bytes;
+  if (ks < bytes || vs < bytes) return set_error(R4Q_ERR_ARG, "%s: page strides below a page's %ld bytes", what, bytes);
+  if (!aligned(c->k_pages, 16) || !aligned(c->v_pages, 16) || ks % 16 || vs % 16)
+    return set_error(R4Q_ERR_ALIGN, "%s: pages must be 16-byte aligned", what);
+  *out = PagedView{(uint8_t*)c->k_pages, (uint8_t*)c->v_pages, ks, vs, c->n_pages, c->page, c->Hk, c->table,
+                   c->ld_table, c->seqs, c->max_blocks, c->k_scale, c->v_scale};
+  return R4Q_OK;
+}
+
+}  // namespace r4q
+
+using namespace r4q;
+
+extern "C" int r4q_paged_kv_write(const void* q, long ldq, const void* k, long ldk, const void* v, long ldv,
+                                  const void* q_norm_w, const void* k_norm_w, const void* cos_tab,
+                                  const void* sin_tab, long tab_stride, long tab_rows, void* q_out, long ldqo,
+                                  void* k_out, long ldko, const r4q_paged_cache* cache, const int* rows,
+                                  const long long* pos, int M, int H, float eps, int flags, void* stream) {
+  WriteArgs a{};
+  int st = paged_view("paged_kv_write", cache, &a.c);
+  if (st) return st;
+  const bool has_q = q && H > 0;
+  if (M < 0 || H < 0) return set_error(R4Q_ERR_ARG, "paged_kv_write: bad shape M=%d H=%d", M, H);
+  if (M == 0) return R4Q_OK;
+  if (!k || !v || !pos) return set_error(R4Q_ERR_ARG, "paged_kv_write: null k, v or pos");
+  if (has_q && !q_out) return set_error(R4Q_ERR_ARG, "paged_kv_write: q without q_out");
+  if (!rows && M > a.c.seqs)
+    return set_error(R4Q_ERR_ARG, "paged_kv_write: %d tokens for %d sequences need rows", M, a.c.seqs);
+  if (flags & ~(R4Q_HEAD_NORM | R4Q_HEAD_ROPE | R4Q_KV_FULL_RANGE))
+    return set_error(R4Q_ERR_ARG, "paged_kv_write: unknown flags %d", flags);
+  if ((flags & R4Q_HEAD_NORM) && ((has_q && !q_norm_w) || !k_norm_w))
+    return set_error(R4Q_ERR_ARG, "paged_kv_write: norm weights required");
+  if ((flags & R4Q_HEAD_ROPE) && (!cos_tab || !sin_tab || tab_rows < 1 || tab_stride < kHeadDim / 2))
+    return set_error(R4Q_ERR_ARG, "paged_kv_write: rope tables required (rows %ld, stride %ld)", tab_rows, tab_stride);
+  const long kd = (long)a.c.Hk * kHeadDim, qd = (long)H * kHeadDim;
+  if (M > 1 && (ldk < kd || ldv < kd || (k_out && ldko < kd) || (has_q && (ldq < qd || ldqo < qd))))
+    return set_error(R4Q_ERR_ARG, "paged_kv_write: row strides below the heads of a token");
+  const bool rope = flags & R4Q_HEAD_ROPE, norm = flags & R4Q_HEAD_NORM;
+  if (!aligned(k, 16) || !aligned(v, 16) || ldk % 8 || ldv % 8 || (k_out && (!aligned(k_out, 16) || ldko % 8)) ||
+      (has_q && (!aligned(q, 16) || !aligned(q_out, 16) || ldq % 8 || ldqo % 8)) ||
+      (rope && (!aligned(cos_tab, 16) || !aligned(sin_tab, 16) || tab_stride % 8)) ||
+      (norm && (!aligned(k_norm_w, 16) || (has_q && !aligned(q_norm_w, 16)))))
+    return set_error(R4Q_ERR_ALIGN, "paged_kv_write: 16-byte aligned pointers and strides in multiples of 8 needed");
+  a.q = (const __half*)q; a.k = (const __half*)k; a.v = (const __half*)v;
+  a.ldq = ldq; a.ldk = ldk; a.ldv = ldv;
+  a.qw = (const __half*)q_norm_w; a.kw = (const __half*)k_norm_w;
+  a.cos_tab = (const __half*)cos_tab; a.sin_tab = (const __half*)sin_tab;
+  a.tab_stride = tab_stride; a.tab_rows = tab_rows;
+  a.q_out = (__half*)q_out; a.k_out = (__half*)k_out; a.ldqo = ldqo; a.ldko = ldko;
+  a.rows = rows; a.pos = pos;
+  a.M = M; a.H = has_q ? H : 0; a.eps = eps; a.flags = flags;
+  a.groups = (a.H + 2 * a.c.Hk + kHeads - 1) / kHeads;
+  const long warps = (long)M * a.groups;
+  if ((warps + 7) / 8 > 0x7fffffffL) return set_error(R4Q_ERR_ARG, "paged_kv_write: M * heads too large");
+  paged_write_kernel<<<(unsigned)((warps + 7) / 8), 256, 0, (cudaStream_t)stream>>>(a);
+  return check_launch("paged_write_kernel");
+}
+
+extern "C" int r4q_kv_copy_pages(void* pool, long outer, long outer_stride, long page_stride, long page_bytes,
+                                 int n_pages, const int* src, const int* dst, int n, void* stream) {
+  if (n < 0 || outer < 0 || (n && (!pool || !src || !dst)) || n_pages < 1 || page_bytes < 16)
+    return set_error(R4Q_ERR_ARG, "kv_copy_pages: bad arguments (n %d, pools %ld, pages %d)", n, outer, n_pages);
+  if (page_stride < page_bytes || (outer > 1 && outer_stride < page_bytes))
+    return set_error(R4Q_ERR_ARG, "kv_copy_pages: strides below a page's %ld bytes", page_bytes);
+  if (!aligned(pool, 16) || page_bytes % 16 || page_stride % 16 || outer_stride % 16)
+    return set_error(R4Q_ERR_ALIGN, "kv_copy_pages: pool, page size and strides must be multiples of 16 bytes");
+  if (outer > 65535) return set_error(R4Q_ERR_ARG, "kv_copy_pages: %ld pools (at most 65535)", outer);
+  std::vector<uint8_t> seen(n ? n_pages : 0, 0);     // 1: read, 2: written
+  for (int i = 0; i < n; ++i) {
+    if (src[i] < 0 || src[i] >= n_pages || dst[i] < 0 || dst[i] >= n_pages)
+      return set_error(R4Q_ERR_ARG, "kv_copy_pages: move %d (%d -> %d) outside the pool of %d pages", i, src[i],
+                       dst[i], n_pages);
+    if (seen[dst[i]] & 2) return set_error(R4Q_ERR_ARG, "kv_copy_pages: page %d is written twice", dst[i]);
+    seen[src[i]] |= 1;
+    seen[dst[i]] |= 2;
+  }
+  for (int i = 0; i < n; ++i)
+    if (seen[src[i]] == 3) return set_error(R4Q_ERR_ARG, "kv_copy_pages: page %d is both read and written", src[i]);
+  if (n == 0 || outer == 0) return R4Q_OK;
+  for (int at = 0; at < n; at += kMaxMoves) {
+    const int part = n - at < kMaxMoves ? n - at : kMaxMoves;
+    Moves mv;
+    memcpy(mv.src, src + at, part * sizeof(int));
+    memcpy(mv.dst, dst + at, part * sizeof(int));
+    copy_pages_kernel<<<dim3(part, (unsigned)outer), 256, 0, (cudaStream_t)stream>>>(
+        (uint8_t*)pool, outer_stride, page_stride, page_bytes, mv);
+    const int st = check_launch("copy_pages_kernel");
+    if (st) return st;
+  }
+  return R4Q_OK;
+}
+
+extern "C" int r4q_kv_table_set(int* table, long ld, int rows, int cols, const int* r, const int* c, const int* v,
+                                int n, void* stream) {
+  if (n < 0 || rows < 0 || cols < 0 || ld < cols || (n && (!table || !r || !c || !v)))
+    return set_error(R4Q_ERR_ARG, "kv_table_set: bad arguments (n %d, table %d x %d)", n, rows, cols);
+  for (int i = 0; i < n; ++i)
+    if (r[i] < 0 || r[i] >= rows || c[i] < 0 || c[i] >= cols)
+      return set_error(R4Q_ERR_ARG, "kv_table_set: cell %d (%d, %d) outside the table of %d x %d", i, r[i], c[i], rows,
+                       cols);
+  for (int at = 0; at < n; at += kMaxCells) {
+    const int part = n - at < kMaxCells ? n - at : kMaxCells;
+    Cells cells;
+    memcpy(cells.r, r + at, part * sizeof(int));
+    memcpy(cells.c, c + at, part * sizeof(int));
+    memcpy(cells.v, v + at, part * sizeof(int));
+    table_set_kernel<<<1, 256, 0, (cudaStream_t)stream>>>(table, ld, part, cells);
+    const int st = check_launch("table_set_kernel");
+    if (st) return st;
+  }
+  return R4Q_OK;
+}
+
+extern "C" int r4q_paged_status(int clear) {
+  int a = 0, b = 0;
+  const int zero = 0;
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&a, g_write_status, sizeof(int));
+  if (e == cudaSuccess && a && clear) e = cudaMemcpyToSymbol(g_write_status, &zero, sizeof(int));
+  if (e == cudaSuccess) e = paged_attn_status(clear, &b);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(R4Q_ERR_CUDA, "paged_status: %s", cudaGetErrorString(e));
+  }
+  if ((a | b) & kPagedBadPage)
+    return set_error(R4Q_ERR_PAGE, "a paged %s met a row, position or page id outside the cache since the last check",
+                     a & kPagedBadPage ? "write" : "attention");
+  if ((a | b) & kPagedTimeout)
+    return set_error(R4Q_ERR_TIMEOUT, "a bounded wait of the paged attention gave up since the last check");
+  return R4Q_OK;
+}

@@ -62,6 +62,14 @@ class ModelDesc(C.Structure):
         ("lm_w", C.c_void_p), ("lm_s", C.c_void_p), ("lm_n", C.c_int), ("tp_rank", C.c_int),
         ("tp_size", C.c_int), ("comm", C.c_void_p)]
 
+
+class PagedCache(C.Structure):
+    """r4q_paged_cache (include/r4q.h)."""
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("k_stride", C.c_long), ("v_stride", C.c_long),
+                ("n_pages", C.c_int), ("page", C.c_int), ("Hk", C.c_int), ("table", C.c_void_p),
+                ("ld_table", C.c_long), ("seqs", C.c_int), ("max_blocks", C.c_int), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p)]
+
 _SIGS = {
     "r4q_last_error": (C.c_char_p, []),
     "r4q_version": (i32, []),
@@ -90,6 +98,14 @@ _SIGS = {
     "r4q_silu_mul": (i32, [vp, i64, vp, i64, i32, i32, vp]),
     "r4q_dequant_int8": (i32, [vp, vp, vp, i32, i32, vp]),
     "r4q_kv_write_rows": (i32, [vp, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp]),
+    "r4q_paged_kv_write": (i32, [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, i64, i64, vp, i64, vp, i64,
+                                 C.POINTER(PagedCache), vp, vp, i32, i32, f32, i32, vp]),
+    "r4q_paged_flash_decode_workspace_bytes": (sz_t, [i32, i32, i32, i32, i32]),
+    "r4q_paged_flash_decode": (i32, [vp, i64, C.POINTER(PagedCache), vp, vp, i64, i32, i32, i32, vp, sz_t, vp]),
+    "r4q_paged_status": (i32, [i32]),
+    "r4q_kv_copy_pages": (i32, [vp, i64, i64, i64, i64, i32, vp, vp, i32, vp]),
+    "r4q_kv_table_set": (i32, [vp, i64, i32, i32, vp, vp, vp, i32, vp]),
+    "r4q_token_logprobs": (i32, [vp, i32, i64, vp, i32, i32, i32, vp, vp, vp, vp, vp, vp]),
     "r4q_moe_route": (i32, [vp, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
     "r4q_norm_fwht_rows": (i32, [vp, vp, i32, vp, f32, vp, i32, i32, vp]),
     "r4q_moe_router": (i32, [vp, vp, i32, vp, f32, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp,
@@ -142,4 +158,8 @@ def call(name: str, *args) -> None:
 PRO_NONE, PRO_FWHT, PRO_SILU_FWHT, PRO_RMSNORM_FWHT = 0, 1, 2, 3
 W_INT4, W_INT8, W_FP16 = 0, 1, 2
 HEAD_NORM, HEAD_ROPE, HEAD_KV = 1, 2, 4
+KV_FULL_RANGE = 8
 ATTN_FWHT = 1
+# element types of r4q_token_logprobs
+T_F16, T_BF16, T_F32 = 0, 1, 2
+MAX_TOP = 32

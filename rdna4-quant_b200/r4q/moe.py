@@ -77,11 +77,21 @@ class MoEDecoder:
     E / world experts, and the fp32 partial sums of the experts' weighted
     outputs are all-reduced over NVLink (r4q_comm_allreduce_f32, rank order)
     before the residual — so each token's expert outputs reach every rank in
-    one exchange of B x hidden fp32 per layer."""
+    one exchange of B x hidden fp32 per layer.
 
-    def __init__(self, model: dict, cfg: dict, batch: int = 1, comm=None):
+    With ``pages`` (r4q.paged.PagedKVCache of at least ``batch`` sequences) K
+    and V go to the pages of sequences 0 .. batch - 1 instead of the model's
+    contiguous caches, and every row has its own position: sequences of
+    different lengths, forks that share a prefix, idle rows.  Positions a step
+    writes must have been reserved (``pages.extend``)."""
+
+    def __init__(self, model: dict, cfg: dict, batch: int = 1, comm=None, pages=None):
         self.m, self.cfg, self.B = model, cfg, batch
         self.comm = comm
+        self.pages = pages
+        if pages is not None and (pages.layers != cfg['num_layers'] or pages.table.shape[0] < batch):
+            raise ValueError(f"paged cache of {pages.layers} layers and {pages.table.shape[0]} sequences for "
+                             f"{cfg['num_layers']} layers and batch {batch}")
         dev = model['embed'].device
         self.dev = dev
         D, H, Hk, hd = cfg['hidden'], cfg['num_heads'], cfg['num_kv_heads'], cfg['head_dim']
@@ -102,6 +112,7 @@ class MoEDecoder:
         self.ss_h = torch.zeros(D // 16, B, dtype=torch.float32, device=dev)
         self.logits = torch.zeros(B, cfg['vocab'], **f16)
         self.seq = torch.ones(B, dtype=torch.int64, device=dev)
+        self.pos = torch.zeros(B, dtype=torch.int64, device=dev)
         W, rk = (comm.world, comm.rank) if comm is not None else (1, 0)
         if E % W:
             raise ValueError(f"{E} experts do not split over {W} ranks")
@@ -132,9 +143,18 @@ class MoEDecoder:
             else:
                 ops.gemv('int4', hin, m['qkv_w'][li], m['qkv_s'][li], qkv_n, D, prologue=L.PRO_RMSNORM_FWHT,
                          out=self.qkv, norm_w=m['in_norm_w'][li], eps=eps, ss_in=None if li == 0 else self.ss_h)
-            ops.attn_decode_fused(self.qkv, m['k_caches'][li], m['v_caches'][li], m['q_norm_w'][li],
-                                  m['k_norm_w'][li], m['rope_cos'], m['rope_sin'], H, Hk, 0, fwht=True, eps=eps,
-                                  out=self.attn, seq_dev=self.seq)
+            if self.pages is None:
+                ops.attn_decode_fused(self.qkv, m['k_caches'][li], m['v_caches'][li], m['q_norm_w'][li],
+                                      m['k_norm_w'][li], m['rope_cos'], m['rope_sin'], H, Hk, 0, fwht=True, eps=eps,
+                                      out=self.attn, seq_dev=self.seq)
+            else:
+                q, k, v = (self.qkv[:, a * hd:(a + n) * hd].view(self.B, n, hd)
+                           for a, n in ((0, H), (H, Hk), (H + Hk, Hk)))
+                ops.paged_kv_write(k, v, *self.pages.pages(li), self.pages.table, self.pos, q=q,
+                                   q_w=m['q_norm_w'][li], k_w=m['k_norm_w'][li], cos=m['rope_cos'],
+                                   sin=m['rope_sin'], q_out=q, eps=eps, **self.pages.codec(li))
+                ops.paged_flash_decode(q, *self.pages.pages(li), self.pages.table, self.seq, fwht=True,
+                                       out=self.attn, **self.pages.scales(li))
             if big:
                 ops.gemm(self.attn.view(self.B, H * hd), m['o_w'][li], m['o_s'][li], D, out=self.o16)
                 ops.residual_f16(self.o16, hin, self.r, ss_out=self.ss_post)
@@ -161,11 +181,28 @@ class MoEDecoder:
             ops.gemv('fp16', self.h, m['lm_w'], None, c['vocab'], D, prologue=L.PRO_RMSNORM_FWHT,
                      out=self.logits, norm_w=m['final_norm_w'], eps=eps)
 
-    def step(self, hidden: torch.Tensor, pos: int, use_graph: bool = True) -> torch.Tensor:
+    def step(self, hidden: torch.Tensor, pos, use_graph: bool = True) -> torch.Tensor:
         """hidden fp16 [B, D] at position pos -> logits [B, vocab] (the step's
-        buffer; copy it before the next step).  K/V of pos go to the caches."""
+        buffer; copy it before the next step).  K/V of pos go to the caches.
+        With a paged cache pos may be a sequence of B positions; a row at
+        position -1 is idle (nothing is written for it, its logits mean nothing)."""
+        if self.pages is None:
+            pos = int(pos)
+        else:
+            pos = pos.tolist() if isinstance(pos, torch.Tensor) else pos
+            pos = [int(p) for p in pos] if hasattr(pos, '__iter__') else [int(pos)] * self.B
+            if len(pos) != self.B:
+                raise ValueError(f"{len(pos)} positions for a batch of {self.B}")
+            for b, p in enumerate(pos):
+                if not -1 <= p < self.pages.lengths[b] or p >= self.m['rope_cos'].shape[0]:
+                    raise ValueError(f"row {b}: position {p} outside the {self.pages.lengths[b]} reserved ones or "
+                                     f"the {self.m['rope_cos'].shape[0]} rows of the RoPE tables")
         self.h_in.copy_(hidden.reshape(self.B, -1))
-        self.seq.fill_(int(pos) + 1)
+        if self.pages is None:
+            self.seq.fill_(pos + 1)
+        else:
+            self.pos.copy_(torch.tensor(pos, dtype=torch.int64))
+            torch.add(self.pos, 1, out=self.seq)
         if not use_graph:
             self._enqueue()
             return self.logits

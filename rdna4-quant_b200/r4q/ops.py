@@ -3,8 +3,11 @@ per-(device, stream) GEMV workspaces.  Device memory and streams come from
 PyTorch; all arithmetic runs in libr4q.so."""
 from __future__ import annotations
 
+import array
 import ctypes as C
 import threading
+from contextlib import nullcontext
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -68,8 +71,10 @@ def check_status(dev: torch.device | int | None = None, clear: bool = True) -> N
     """Raise ``R4QError`` (code R4Q_ERR_TIMEOUT) if a bounded device-side wait
     of a GEMV, GEMM or attention kernel gave up since the last check on this
     device: the outputs of those kernels are then not valid.  Reads the status
-    word of every workspace these wrappers hold for the device, and of the
-    allocation-free GEMV's static scratch (synchronises each stream)."""
+    word of every workspace these wrappers hold for the device, of the
+    allocation-free GEMV's static scratch and of the paged kernels, which also
+    report a page id, position or row outside the cache (R4Q_ERR_PAGE).
+    Synchronises the device."""
     if dev is None:
         dev = torch.cuda.current_device()
     idx = dev if isinstance(dev, int) else (dev.index if dev.index is not None else torch.cuda.current_device())
@@ -84,6 +89,9 @@ def check_status(dev: torch.device | int | None = None, clear: bool = True) -> N
         st = L.LIB.r4q_ws_status(None, 1 if clear else 0, None)
         if st != 0 and err is None:
             err = L.R4QError(st, "r4q_ws_status(noalloc scratch)", L.last_error())
+        st = L.LIB.r4q_paged_status(1 if clear else 0)
+        if st != 0 and err is None:
+            err = L.R4QError(st, "r4q_paged_status", L.last_error())
     if err is not None:
         raise err
 
@@ -400,3 +408,241 @@ def residual_f16(a: torch.Tensor, res: torch.Tensor | None, out: torch.Tensor, s
     B, D = a.shape
     L.call("r4q_residual_f16", a.data_ptr(), _ptr(res), out.data_ptr(), _ptr(ss_out), B, D, stream_handle(dev))
     return out
+
+
+# ------------------------------------------------------------- paged KV cache ---
+def _on(dev: torch.device):
+    """Makes dev the current device for a launch on one of its streams."""
+    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _heads(t: torch.Tensor, name: str, rows: Optional[int] = None, heads: Optional[int] = None,
+           out: bool = False) -> torch.Tensor:
+    """t as fp16 [rows, heads, 128] with its heads side by side and any row
+    stride; an input laid out otherwise is copied, an output refused."""
+    if t.dtype != torch.float16:
+        raise TypeError(f"{name} must be float16")
+    if t.dim() != 3 or t.shape[2] != 128 or (rows is not None and t.shape[0] != rows) or \
+            (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name} must be [{rows or 'rows'}, {heads or 'heads'}, 128], got {tuple(t.shape)}")
+    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != 128) or
+                      (t.shape[0] > 1 and t.stride(0) < t.shape[1] * 128)):
+        if out:
+            raise ValueError(f"{name} must hold the heads of a row side by side")
+        t = t.contiguous()
+    return t
+
+
+def _vector(t: torch.Tensor, name: str, dtype: torch.dtype, n: int) -> torch.Tensor:
+    if t.dtype != dtype or tuple(t.shape) != (n,):
+        raise ValueError(f"{name} must be {str(dtype)[6:]} [{n}], got {str(t.dtype)[6:]} {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _paged_cache(k_pages, v_pages, block_table, k_scale, v_scale) -> L.PagedCache:
+    if k_pages.dtype != torch.uint8 or v_pages.dtype != torch.uint8:
+        raise TypeError("pages must be uint8 (FP8 E4M3 bytes)")
+    if k_pages.dim() != 4 or k_pages.shape[3] != 128 or v_pages.shape != k_pages.shape:
+        raise ValueError("k_pages and v_pages must be [pages, kv heads, page, 128] of one shape, got "
+                         f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    P, Hk, page, _ = k_pages.shape
+    for t in (k_pages, v_pages):
+        if t.stride(3) != 1 or t.stride(2) != 128 or (Hk > 1 and t.stride(1) != page * 128):
+            raise ValueError("each page must be contiguous [kv heads, page, 128]")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2:
+        raise TypeError("block_table must be int32 [sequences, blocks]")
+    S, nb = block_table.shape
+    if nb and block_table.stride(1) != 1:
+        raise ValueError("block_table rows must be contiguous")
+    for s in (k_scale, v_scale):
+        if s is not None and (s.dtype != torch.float32 or tuple(s.shape) != (Hk,) or not s.is_contiguous()):
+            raise ValueError(f"k_scale and v_scale must be float32 [{Hk}], one per kv head")
+    return L.PagedCache(k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0) if P > 1 else 0,
+                        v_pages.stride(0) if P > 1 else 0, P, page, Hk, block_table.data_ptr(),
+                        block_table.stride(0) if S > 1 else nb, S, nb, _ptr(k_scale), _ptr(v_scale))
+
+
+def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                   block_table: torch.Tensor, positions: torch.Tensor, *, rows: Optional[torch.Tensor] = None,
+                   q: Optional[torch.Tensor] = None, q_w=None, k_w=None, cos=None, sin=None, q_out=None, k_out=None,
+                   k_scale=None, v_scale=None, eps: float = 1e-6, full_range: bool = False) -> Optional[torch.Tensor]:
+    """New tokens into the pages of a paged FP8 cache (r4q_paged_kv_write).
+
+    k, v fp16 [M, Hk, 128] (views of a wider row are fine); pages uint8
+    [P, Hk, page, 128]; block_table int32 [sequences, blocks]; token m goes to
+    ``positions[m]`` (int64; negative: padding, skipped) of sequence ``rows[m]``
+    (int32; default m).  With ``k_w`` (and ``q_w``) the heads of k (and q) are
+    RMS-normalised, with ``cos`` / ``sin`` (fp16 [rows, 64]) rotated at their
+    position first; q [M, H, 128] then comes back in ``q_out`` (default: a new
+    tensor, undefined in the rows of padding; q itself for in place) and k in
+    ``k_out`` if given.  ``k_scale`` / ``v_scale``: fp32 [Hk], stored byte =
+    enc(x / scale), the bytes of the contiguous cache; ``full_range`` keeps
+    256 .. 448 apart, which its codec stores as 448.  Rows, positions and page ids out of range write nothing
+    and are reported by ``check_status``."""
+    ts = [t for t in (k, v, k_pages, v_pages, block_table, positions, rows, q, q_w, k_w, cos, sin, q_out, k_out,
+                      k_scale, v_scale) if t is not None]
+    dev = _require_cuda(*ts)
+    cache = _paged_cache(k_pages, v_pages, block_table, k_scale, v_scale)
+    Hk = cache.Hk
+    k = _heads(k, "k", heads=Hk)
+    M = k.shape[0]
+    v = _heads(v, "v", M, Hk)
+    positions = _vector(positions, "positions", torch.int64, M)
+    if rows is not None:
+        rows = _vector(rows, "rows", torch.int32, M)
+    H, flags, tab = 0, L.KV_FULL_RANGE if full_range else 0, (0, 0)
+    if q is not None:
+        q = _heads(q, "q", M)
+        H = q.shape[1]
+        q_out = torch.empty(M, H, 128, dtype=torch.float16, device=dev) if q_out is None else \
+            _heads(q_out, "q_out", M, H, out=True)
+    elif q_out is not None or q_w is not None:
+        raise ValueError("q_out and q_w need q")
+    if k_out is not None:
+        k_out = _heads(k_out, "k_out", M, Hk, out=True)
+    if k_w is not None or q_w is not None:
+        if k_w is None or (q is not None and q_w is None):
+            raise ValueError("the norm needs a weight for q and for k")
+        for w in (q_w, k_w):
+            if w is not None and (w.dtype != torch.float16 or tuple(w.shape) != (128,) or not w.is_contiguous()):
+                raise ValueError("norm weights must be float16 [128]")
+        flags |= L.HEAD_NORM
+    if cos is not None or sin is not None:
+        for t in (cos, sin):
+            if t is None or t.dtype != torch.float16 or t.dim() != 2 or t.shape[1] < 64 or t.stride(1) != 1 or \
+                    t.shape != cos.shape or t.stride(0) != cos.stride(0):
+                raise ValueError("cos and sin must be float16 [rows, 64] of one layout")
+        flags |= L.HEAD_ROPE
+        tab = (cos.stride(0) if cos.shape[0] > 1 else 64, cos.shape[0])
+    with _on(dev):
+        L.call("r4q_paged_kv_write", _ptr(q), 0 if q is None else _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v),
+               _ptr(q_w), _ptr(k_w), _ptr(cos), _ptr(sin), tab[0], tab[1], _ptr(q_out),
+               0 if q_out is None else _ld(q_out), _ptr(k_out), 0 if k_out is None else _ld(k_out), C.byref(cache),
+               _ptr(rows), positions.data_ptr(), M, H, float(eps), flags, stream_handle(dev))
+    return q_out
+
+
+def paged_flash_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                       seq_lens: torch.Tensor, *, k_scale=None, v_scale=None, fwht: bool = False,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per sequence over a paged FP8 cache: q fp16
+    [B, H, 128], pages uint8 [P, Hk, page, 128], block_table int32
+    [sequences >= B, blocks], seq_lens int64 [B] -> o fp16 [B, H, 128]
+    (``flash_decode`` over a contiguous cache).  A sequence of length 0 gives
+    zeros.  Page ids outside the pool read as zeros and lengths beyond the
+    table are cut; ``check_status`` reports both.  The workspace comes from
+    torch's allocator at every call, so calls on several streams and captured
+    graphs share nothing."""
+    dev = _require_cuda(q, k_pages, v_pages, block_table, seq_lens, *(t for t in (k_scale, v_scale, out) if t is not None))
+    q = _heads(q, "q")
+    B, H, _ = q.shape
+    cache = _paged_cache(k_pages, v_pages, block_table, k_scale, v_scale)
+    seq_lens = _vector(seq_lens, "seq_lens", torch.int64, B)
+    o = torch.empty(B, H, 128, dtype=torch.float16, device=dev) if out is None else _heads(out, "out", B, H, out=True)
+    with _on(dev):
+        need = L.LIB.r4q_paged_flash_decode_workspace_bytes(B, H, cache.Hk, cache.page, cache.max_blocks)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        L.call("r4q_paged_flash_decode", q.data_ptr(), _ld(q), C.byref(cache), seq_lens.data_ptr(), o.data_ptr(),
+               _ld(o), B, H, L.ATTN_FWHT if fwht else 0, _ptr(ws), need, stream_handle(dev))
+    return o
+
+
+def _host_ints(*lists) -> list:
+    """Host sequences or CPU tensors of equal length as arrays of C ints."""
+    out = []
+    for x in lists:
+        if isinstance(x, torch.Tensor):
+            if x.is_cuda:
+                raise ValueError("page lists are host data (lists or CPU tensors)")
+            x = x.tolist()
+        try:
+            out.append(array.array('i', x))
+        except OverflowError:
+            raise ValueError("page lists must hold 32-bit integers") from None
+        if len(out[-1]) != len(out[0]):
+            raise ValueError("page lists must have one length")
+    return out
+
+
+def kv_copy_pages(pool: torch.Tensor, src, dst) -> None:
+    """pool[..., dst[i], :, :, :] = pool[..., src[i], :, :, :] for every i, in one
+    launch over all leading dimensions (layers, K and V): pool uint8
+    [..., P, Hk, page, 128], contiguous; src and dst host lists.  A page may be
+    copied to several places, but not written twice, nor both read and
+    written (r4q_kv_copy_pages)."""
+    dev = _require_cuda(pool)
+    if pool.dtype != torch.uint8 or pool.dim() < 4 or not pool.is_contiguous():
+        raise ValueError("pool must be uint8 [..., pages, kv heads, page, 128] and contiguous")
+    s, d = _host_ints(src, dst)
+    P = pool.shape[-4]
+    page_bytes = pool.shape[-3] * pool.shape[-2] * pool.shape[-1]
+    outer = pool.numel() // max(1, P * page_bytes)
+    if not pool.numel():
+        raise ValueError("empty pool")
+    with _on(dev):
+        L.call("r4q_kv_copy_pages", pool.data_ptr(), outer, P * page_bytes, page_bytes, page_bytes, P,
+               s.buffer_info()[0], d.buffer_info()[0], len(s), stream_handle(dev))
+
+
+def kv_table_set(table: torch.Tensor, rows, cols, values) -> None:
+    """table[rows[i], cols[i]] = values[i] in stream order, from host lists
+    (r4q_kv_table_set): table int32 [sequences, blocks] on the device; no cell twice."""
+    dev = _require_cuda(table)
+    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("table must be int32 [sequences, blocks] with contiguous rows")
+    r, c, v = _host_ints(rows, cols, values)
+    with _on(dev):
+        L.call("r4q_kv_table_set", table.data_ptr(), table.stride(0) if table.shape[0] > 1 else table.shape[1],
+               table.shape[0], table.shape[1], r.buffer_info()[0], c.buffer_info()[0], v.buffer_info()[0], len(r),
+               stream_handle(dev))
+
+
+# ----------------------------------------------------------- token likelihoods ---
+class TokenLogprobs(NamedTuple):
+    """Of M rows: log probability (fp32 [M]) and rank (int64 [M], 1 = most
+    likely) of the given tokens, None without tokens; entropy in nats (fp32
+    [M]); the k most likely ids (int64 [M, k]) and their log probabilities."""
+    logprob: Optional[torch.Tensor]
+    rank: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+_LOGIT_TYPES = {torch.float16: L.T_F16, torch.bfloat16: L.T_BF16, torch.float32: L.T_F32}
+
+
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, k: int = 0) -> TokenLogprobs:
+    """Log probabilities of ``tokens`` (int64 [M]) under softmax(logits[M, V])
+    (fp16, bf16 or fp32; rows any stride apart), with their rank, the rows'
+    entropy and the k <= 32 most likely alternatives, in one pass over the
+    logits (r4q_token_logprobs).  Ties go to the lowest id.  A token outside
+    [0, V) gets NaN and rank 0; a row that is no distribution (NaN, +inf, or
+    -inf throughout) gives NaN."""
+    ty = _LOGIT_TYPES.get(logits.dtype)
+    if ty is None:
+        raise TypeError(f"logits must be float16, bfloat16 or float32, not {logits.dtype}")
+    if logits.dim() != 2:
+        raise ValueError("logits must be [rows, vocabulary]")
+    dev = _require_cuda(logits) if tokens is None else _require_cuda(logits, tokens)
+    M, V = logits.shape
+    if V < 1 or not 0 <= k <= min(V, L.MAX_TOP):
+        raise ValueError(f"k must be in [0, {min(V, L.MAX_TOP)}], got {k} (vocabulary {V})")
+    if (V > 1 and logits.stride(1) != 1) or (M > 1 and logits.stride(0) < V):
+        logits = logits.contiguous()
+    if tokens is not None:
+        tokens = _vector(tokens, "tokens", torch.int64, M)
+    f32 = dict(dtype=torch.float32, device=dev)
+    i64 = dict(dtype=torch.int64, device=dev)
+    r = TokenLogprobs(None if tokens is None else torch.empty(M, **f32),
+                      None if tokens is None else torch.empty(M, **i64), torch.empty(M, **f32),
+                      torch.empty(M, k, **i64), torch.empty(M, k, **f32))
+    with _on(dev):
+        L.call("r4q_token_logprobs", logits.data_ptr(), ty, logits.stride(0) if M > 1 else V, _ptr(tokens), M, V, k,
+               _ptr(r.logprob), _ptr(r.rank), r.entropy.data_ptr(), r.top_ids.data_ptr(), r.top_logprobs.data_ptr(),
+               stream_handle(dev))
+    return r

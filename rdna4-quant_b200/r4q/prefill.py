@@ -53,14 +53,20 @@ def linear(x: torch.Tensor, w: torch.Tensor, s, N: int) -> torch.Tensor:
 def prefill_logits(hidden: torch.Tensor, qkv_w, qkv_s, o_w, o_s, gu_w, gu_s, down_w, down_s, in_norm_w,
                    post_norm_w, q_norm_w, k_norm_w, rope_cos, rope_sin, num_heads, num_kv_heads, head_dim,
                    hidden_size, intermediate_size, rms_eps, final_norm_w, lm_w, lm_s, lm_N, k_caches=None,
-                   v_caches=None, batch_row: int = 0, k_scales=None, v_scales=None, last_only: bool = False):
+                   v_caches=None, batch_row: int = 0, k_scales=None, v_scales=None, last_only: bool = False,
+                   pages=None):
     """hidden fp16 [M, D] (embedded prompt) -> logits fp16 [M, lm_N].
 
     With ``k_caches`` / ``v_caches`` (uint8 [B, Hk, max_seq, 128] per layer)
     the prompt's rotated K and V of every layer are written to positions
     0..M-1 of ``batch_row`` (an extension: the reference prefill writes no
-    cache), so decoding can continue at position M.  ``last_only`` returns
-    the logits of the last position only [1, lm_N]."""
+    cache), so decoding can continue at position M.  With ``pages``
+    (r4q.paged.PagedKVCache) they are written to the pages of sequence
+    ``batch_row`` instead, which holds M positions already
+    (``pages.extend({batch_row: M})``).  ``last_only`` returns the logits of
+    the last position only [1, lm_N]."""
+    if pages is not None and k_caches is not None:
+        raise ValueError("prefill_logits: k_caches or pages, not both")
     x = hidden.reshape(-1, int(hidden_size)).contiguous()
     M, D = x.shape
     dev = x.device
@@ -68,13 +74,24 @@ def prefill_logits(hidden: torch.Tensor, qkv_w, qkv_s, o_w, o_s, gu_w, gu_s, dow
     qd, kvd = H * hd, Hk * hd
     qkv_n = qd + 2 * kvd
     pos = torch.arange(M, dtype=torch.int64, device=dev)
+    if pages is not None:
+        if pages.lengths[batch_row] < M or rope_cos.shape[0] < M:
+            raise ValueError(f"sequence {batch_row} holds {pages.lengths[batch_row]} positions and the RoPE tables "
+                             f"{rope_cos.shape[0]}, the prompt {M}")
+        rows = torch.full((M,), int(batch_row), dtype=torch.int32, device=dev)
     normed = ops.rmsnorm(x, in_norm_w[0], rms_eps)
     nl = len(qkv_w)
     for li in range(nl):
         qkv = linear(ops.fwht_rows(normed), qkv_w[li], qkv_s[li], qkv_n)
-        ops.head_norm_rope(qkv, qkv[:, qd:], q_w=q_norm_w[li], k_w=k_norm_w[li], cos=rope_cos, sin=rope_sin,
-                           pos_dev=pos, q_out=qkv, k_out=qkv[:, qd:], B=M, H=H, Hk=Hk, D=hd, ld_in=qkv_n,
-                           ld_out=qkv_n, eps=rms_eps, flags=L.HEAD_NORM | L.HEAD_ROPE)
+        if pages is not None:                  # norm, rotation and page write in one launch
+            qh, kh, vh = (qkv[:, a:a + n * hd].view(M, n, hd) for a, n in ((0, H), (qd, Hk), (qd + kvd, Hk)))
+            ops.paged_kv_write(kh, vh, *pages.pages(li), pages.table, pos, rows=rows, q=qh, q_w=q_norm_w[li],
+                               k_w=k_norm_w[li], cos=rope_cos, sin=rope_sin, q_out=qh, k_out=kh, eps=rms_eps,
+                               **pages.codec(li))
+        else:
+            ops.head_norm_rope(qkv, qkv[:, qd:], q_w=q_norm_w[li], k_w=k_norm_w[li], cos=rope_cos, sin=rope_sin,
+                               pos_dev=pos, q_out=qkv, k_out=qkv[:, qd:], B=M, H=H, Hk=Hk, D=hd, ld_in=qkv_n,
+                               ld_out=qkv_n, eps=rms_eps, flags=L.HEAD_NORM | L.HEAD_ROPE)
         if k_caches is not None:
             L.call("r4q_kv_write_rows", qkv[:, qd:].data_ptr(), qkv[:, qd + kvd:].data_ptr(), qkv_n,
                    k_caches[li].data_ptr(), v_caches[li].data_ptr(), M, Hk, hd, int(k_caches[li].shape[2]), 0,

@@ -21,15 +21,30 @@ from __future__ import annotations
 
 import itertools
 import threading
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Callable, Optional, Sequence
 
 import torch
 
 from . import decode
+from . import lib as L
+from . import ops
 from . import prefill as P
 
 _ids = itertools.count(1)
+
+
+@dataclass(frozen=True)
+class TokenLogprob:
+    """Likelihood of one generated token under the model's distribution
+    (softmax of the raw logits, before temperature and top-p): its log
+    probability and rank (1 = most likely), the entropy of the distribution in
+    nats, and the most likely alternatives as (id, log probability) pairs."""
+    token: int
+    logprob: float
+    rank: int
+    entropy: float
+    top: tuple
 
 
 @dataclass
@@ -37,7 +52,10 @@ class Request:
     """One generation request.  ``tokens`` collects the generated ids;
     ``finish_reason`` is None while running, then "stop" (a stop id was
     sampled, and is kept as the last token, as the reference keeps EOS),
-    "length" (max_new_tokens reached) or "cache" (the KV cache is full)."""
+    "length" (max_new_tokens reached) or "cache" (the KV cache is full).
+    ``logprobs``: None, or the number of alternatives (0..32) for which
+    ``token_logprobs`` collects one TokenLogprob per generated token (there
+    before ``on_token`` sees the token)."""
     prompt: Sequence[int]
     max_new_tokens: int = 64
     stop_ids: Sequence[int] = ()
@@ -48,6 +66,8 @@ class Request:
     tokens: list = field(default_factory=list)
     finish_reason: Optional[str] = None
     on_token: Optional[Callable[["Request", int], None]] = None
+    logprobs: Optional[int] = None
+    token_logprobs: list = field(default_factory=list)
 
     @property
     def done(self) -> bool:
@@ -118,6 +138,15 @@ class SlotBackend:
         self.ctx.step_rows(self.hidden, positions, logits_out=self.logits, use_graph=self.use_graph)
         return self.logits
 
+    def logprobs(self, logits: torch.Tensor, tokens: Sequence[int], k: int) -> list:
+        """TokenLogprob of tokens[i] under logits[i] ([rows, vocab]) with the k
+        most likely alternatives (k is cut to the vocabulary)."""
+        toks = torch.as_tensor(list(tokens), dtype=torch.long, device=self.dev)
+        r = ops.token_logprobs(logits, toks, min(int(k), int(logits.shape[1])))
+        cols = [t.tolist() for t in (r.logprob, r.rank, r.entropy, r.top_ids, r.top_logprobs)]
+        return [TokenLogprob(int(t), lp, rk, h, tuple(zip(ids, lps)))
+                for t, lp, rk, h, ids, lps in zip(tokens, *cols)]
+
 
 class BatchedEngine:
     """Slots, admission and retirement around a backend (``SlotBackend``).
@@ -149,6 +178,11 @@ class BatchedEngine:
             raise ValueError(f"prompt of {len(r.prompt)} tokens does not fit the KV cache ({self.max_seq})")
         if r.max_new_tokens < 1:
             raise ValueError("max_new_tokens must be >= 1")
+        if r.logprobs is not None:
+            if not 0 <= r.logprobs <= L.MAX_TOP:
+                raise ValueError(f"logprobs must be in [0, {L.MAX_TOP}], got {r.logprobs}")
+            if not hasattr(self.be, 'logprobs'):
+                raise ValueError("this backend gives no log probabilities")
         with self.lock:
             self.queue.append(r)
         return r
@@ -188,7 +222,10 @@ class BatchedEngine:
                 self.slots[s] = r
                 lg = self.be.prefill(s, r.prompt)
                 self.pos[s] = len(r.prompt)
-                self._emit(s, r, sample(lg, r.temperature, r.top_p, self._gen(r)))
+                tok = sample(lg, r.temperature, r.top_p, self._gen(r))
+                if r.logprobs is not None:
+                    r.token_logprobs += self.be.logprobs(lg.reshape(1, -1), [tok], r.logprobs)
+                self._emit(s, r, tok)
 
     @property
     def active(self) -> int:
@@ -208,9 +245,18 @@ class BatchedEngine:
             picks = dict(zip(greedy, am)) if greedy else {}
             for s in rows:
                 r = self.slots[s]
-                tok = picks[s] if s in picks else sample(logits[s], r.temperature, r.top_p, self._gen(r))
+                if s not in picks:
+                    picks[s] = sample(logits[s], r.temperature, r.top_p, self._gen(r))
+            wanted = [s for s in rows if self.slots[s].logprobs is not None]
+            if wanted:                     # one call for the rows that want them, with the largest k
+                lps = self.be.logprobs(logits if len(wanted) == self.batch else logits[wanted],
+                                       [picks[s] for s in wanted], max(self.slots[s].logprobs for s in wanted))
+                for s, lp in zip(wanted, lps):
+                    r = self.slots[s]
+                    r.token_logprobs.append(replace(lp, top=lp.top[:r.logprobs]))
+            for s in rows:
                 self.pos[s] += 1
-                self._emit(s, r, tok)
+                self._emit(s, self.slots[s], picks[s])
             self.steps += 1
             return len(rows)
 
