@@ -1,68 +1,546 @@
-// Attention of one new token over the paged FP8 KV cache.
+// Attention of one new token per sequence over the paged FP8 KV cache, split
+// over the cache's length and joined.
 //
-// o = sum_j p_j V_j / sum_j p_j with p_j = exp2(s_j - m), s_j the score in the
-// log2 domain and m the running maximum: one pass over K and V.
+//   o = sum_j p_j V_j / sum_j p_j,   p_j = 2^(s_j - m),   s_j = q.K_j ks log2(e) / sqrt(128)
 //
-// One CTA per (sequence, query head), positions strided over its 8 warps, a
-// lane holds 4 of the 128 elements; the warps join through shared memory.
+// in one pass over K and V with the running maximum m; parts of a sequence join
+// as (m, l, O): M = max m, weights 2^(m - M).
+//
+// Bound: HBM, 256 bytes per position and kv head; the arithmetic (tensor cores
+// through m16n8k16, FP8 -> f16 by the hardware pair conversion) has to hide
+// under it.
+//
+// Split.  The work is one list of 32-position tiles, ordered by (sequence, kv
+// head, group of 8 query heads, tile); its length comes from the lengths on the
+// device.  Every CTA takes an equal run of it and every warp of the CTA an equal
+// run of that, whatever the lengths are: a batch of one long and many short
+// sequences loads the SMs as evenly as an even one.  A (sequence, head) that lies
+// inside one warp's run is finished in its registers; parts join in shared
+// memory within a CTA, and through the workspace across CTAs, in a second small
+// kernel (programmatic dependent launch) that reads them in list order: no
+// atomics and no state between calls, so results repeat bit for bit and nothing
+// is shared by calls that run at once.
+//
+// Per warp.  A ring of K/V tiles filled by TMA (128-byte swizzle, one box per
+// tile, or two of 16 positions when the page is no multiple of 32); lane 0
+// issues, the coordinates of the next 32 tiles are worked out by the 32 lanes
+// together, so that the block-table reads do not wait for one another.  Pages
+// that do not exist are loaded from behind the pool, i.e. as zeros.
+//
+// Precision.  q, K and V enter the products exactly (f16); a weight enters as
+// two f16 numbers, its rounding and what that left, which takes no extra
+// instruction: query heads fill 8 of the 16 rows of a product, the remainders the
+// other 8.  Scores, maxima, sums and O are fp32.  One rounding to f16 at the end.
+#include <cuda.h>
+
+#include <mutex>
+
 #include "paged.cuh"
 #include "r4q_common.cuh"
+#include "tma_dev.cuh"
 
 namespace r4q {
 namespace {
 
 __device__ int g_attn_status;
-constexpr int kWarps = 8;
 
-__global__ void __launch_bounds__(kWarps * 32)
-    paged_attn_kernel(const __half* q, long ldq, const PagedView c, const long long* seq_lens, __half* o, long ldo,
-                      int Hg, int fwht) {
-  __shared__ float part[kWarps][130];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.x, b = blockIdx.y, kh = h / Hg;
-  const long long cap = (long long)c.max_blocks * c.page;
-  long long seq = seq_lens[b];
-  if (seq > cap || seq < 0) {
-    if (threadIdx.x == 0) atomicOr(&g_attn_status, kPagedBadPage);
-    seq = seq < 0 ? 0 : cap;
-  }
-  float qv[4], acc[4] = {0.f, 0.f, 0.f, 0.f}, m = -1e30f, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) qv[i] = seq ? __half2float(q[(long)b * ldq + (long)h * kHeadDim + 4 * lane + i]) : 0.f;
-  const float scale = (c.k_scale ? c.k_scale[kh] : 1.f) * rsqrtf((float)kHeadDim) * 1.4426950408889634f;
-  for (int p = warp; p < (int)seq; p += kWarps) {
-    const int pg = c.table[(long)b * c.ld_table + p / c.page];
-    const bool ok = pg >= 0 && pg < c.n_pages;
-    if (!ok && lane == 0) atomicOr(&g_attn_status, kPagedBadPage);
-    const long off = ((long)kh * c.page + p % c.page) * kHeadDim + 4 * lane;
-    const uint32_t kw = ok ? *reinterpret_cast<const uint32_t*>(c.k + pg * c.k_stride + off) : 0u;
-    const uint32_t vw = ok ? *reinterpret_cast<const uint32_t*>(c.v + pg * c.v_stride + off) : 0u;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s += qv[i] * fp8_decode((kw >> (8 * i)) & 0xff);
-    s = warp_sum(s) * scale;
-    const float mn = fmaxf(m, s), f = exp2f(m - mn), e = exp2f(s - mn);
-    m = mn;
-    l = l * f + e;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = acc[i] * f + e * fp8_decode((vw >> (8 * i)) & 0xff);
-  }
-  if (lane == 0) part[warp][128] = m, part[warp][129] = l;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) part[warp][4 * lane + i] = acc[i];
-  __syncthreads();
-  if (threadIdx.x >= kHeadDim) return;
-  float M = -1e30f, L = 0.f, O = 0.f;
-  for (int w = 0; w < kWarps; ++w) M = fmaxf(M, part[w][128]);
-  for (int w = 0; w < kWarps; ++w) {
-    const float f = exp2f(part[w][128] - M);
-    L += part[w][129] * f;
-    O += part[w][threadIdx.x] * f;
-  }
-  float r = L > 0.f ? O * ((c.v_scale ? c.v_scale[kh] : 1.f) / L) : 0.f;
-  if (fwht) r = fwht32_lane(r, lane);
-  o[(long)b * ldo + (long)h * kHeadDim + threadIdx.x] = __float2half(r);
+constexpr int kWarps = 8;
+constexpr int kSlots = 2;
+constexpr int kTile = 32;                         // positions per tile
+constexpr int kTileBytes = kTile * kHeadDim;      // of K, and of V
+constexpr int kGroup = 8;                         // query heads per pass over K and V
+constexpr int kPitch = 132;                       // floats of a part's head: O[128], m, l, padding
+constexpr int kPartFloats = kGroup * kPitch;
+constexpr int kMaxBatch = 4096;
+constexpr int kWaitPolls = 1 << 22;
+
+struct AttnArgs {
+  const __half* q;
+  long ldq;
+  PagedView c;
+  const long long* seq_lens;
+  __half* o;
+  long ldo;
+  int B, H, Hg, chunks, fwht;
+  int per_seg;       // a CTA per (sequence, head, group) instead of equal runs
+  int two_boxes;     // 16-position boxes
+  int* header;       // workspace: tiles per CTA, then the prefix sums of tiles [B + 1]
+  float* parts;      // workspace: [CTA][2][kPartFloats]
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
+__device__ __forceinline__ bool wait_full(uint64_t* bar, unsigned parity) {
+  const uint32_t b = smem_u32(bar);
+  for (int i = 0; i < kWaitPolls; ++i) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+                 " selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(b), "r"(parity) : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int row, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row),
+      "r"(page), "r"(smem_u32(bar)) : "memory");
+}
+
+// H32 of the 32-element blocks of a head that a warp holds 4 per lane (4 lane ..).
+__device__ __forceinline__ void fwht32_x4(float (&v)[4], int lane) {
+  float a = v[0] + v[1], b = v[0] - v[1], c = v[2] + v[3], d = v[2] - v[3];
+  v[0] = a + c; v[1] = b + d; v[2] = a - c; v[3] = b - d;
+#pragma unroll
+  for (int s = 1; s < 8; s <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float o = __shfl_xor_sync(0xffffffffu, v[i], s);
+      v[i] = (lane & s) ? o - v[i] : v[i] + o;
+    }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] *= kInvSqrt32;
+}
+
+// A warp joins n parts of one head (part(i): its 132 floats) and gives O, unnormalised, 4 per lane.
+template <typename F>
+__device__ __forceinline__ void join(int n, int lane, F part, float& M, float& L, float (&O)[4]) {
+  M = -1e30f;
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, part(i)[kHeadDim]);
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
+  L = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) O[i] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float* p = part(i);
+    const float f = ex2(p[kHeadDim] - M);
+    const float4 v = *reinterpret_cast<const float4*>(p + 4 * lane);
+    L += p[kHeadDim + 1] * f;
+    O[0] += v.x * f; O[1] += v.y * f; O[2] += v.z * f; O[3] += v.w * f;
+  }
+}
+__device__ __forceinline__ void store_head(const AttnArgs& a, int b, int head, int kh, float L, float (&O)[4],
+                                           int lane) {
+  const float inv = L > 0.f ? (a.c.v_scale ? a.c.v_scale[kh] : 1.f) / L : 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) O[i] *= inv;
+  if (a.fwht) fwht32_x4(O, lane);
+  *reinterpret_cast<uint2*>(a.o + (long)b * a.ldo + (long)head * kHeadDim + 4 * lane) =
+      make_uint2(h2_as_u32(__floats2half2_rn(O[0], O[1])), h2_as_u32(__floats2half2_rn(O[2], O[3])));
+}
+
+__device__ __forceinline__ int seq_of(const AttnArgs& a, int b) {
+  const long long s = a.seq_lens[b], cap = (long long)a.c.max_blocks * a.c.page;
+  return (int)(s < 0 ? 0 : s > cap ? cap : s);
+}
+
+struct Place {                 // of a tile in the list
+  int b, hc, t, T;             // sequence, kv head * chunks + chunk, tile and tiles of the sequence
+};
+__device__ __forceinline__ Place place_of(const int* prefix, int B, int Hc, int x) {
+  const int y = x / Hc;
+  int lo = 0, hi = B;                               // prefix[lo] <= y < prefix[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] <= y) lo = mid; else hi = mid;
+  }
+  const int T = prefix[lo + 1] - prefix[lo], rem = x - prefix[lo] * Hc;
+  return Place{lo, rem / T, rem % T, T};
+}
+
+__global__ void __launch_bounds__(kWarps * 32, 1)
+    paged_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                      const AttnArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem + warp * (kSlots * 2 * kTileBytes);
+  float* part0 = reinterpret_cast<float*>(smem + kWarps * kSlots * 2 * kTileBytes);   // [warp][head, tail][..]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(part0 + kWarps * 2 * kPartFloats);
+  int* meta = reinterpret_cast<int*>(bars + kWarps * kSlots);                          // [warp][head, tail] segment
+  int* wsum = meta + 2 * kWarps;
+  int* prefix = wsum + kWarps;                                                        // [B + 1]
+  uint64_t* wbars = bars + warp * kSlots;
+  const int Hc = a.c.Hk * a.chunks;
+
+  if (lane == 0) {
+    for (int s = 0; s < kSlots; ++s) mbar_init(&wbars[s], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    meta[2 * warp] = meta[2 * warp + 1] = -1;
+  }
+  pdl_wait_trigger();
+
+  // prefix sums of the tiles of the sequences
+  {
+    const int each = (a.B + kWarps * 32 - 1) / (kWarps * 32), b0 = tid * each;
+    int own = 0;
+    bool bad = false;
+    for (int i = 0; i < each; ++i)
+      if (b0 + i < a.B) {
+        const int n = seq_of(a, b0 + i);
+        bad |= n != a.seq_lens[b0 + i];
+        own += (n + kTile - 1) / kTile;
+      }
+    if (bad && blockIdx.x == 0) atomicOr(&g_attn_status, kPagedBadPage);
+    int inc = own;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, inc, s);
+      if (lane >= s) inc += o;
+    }
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    int at = inc - own;
+    for (int w = 0; w < warp; ++w) at += wsum[w];
+    if (tid == 0) prefix[0] = 0;
+    for (int i = 0; i < each; ++i)
+      if (b0 + i < a.B) {
+        at += (seq_of(a, b0 + i) + kTile - 1) / kTile;
+        prefix[b0 + i + 1] = at;
+      }
+    __syncthreads();
+  }
+  const int N = prefix[a.B] * Hc;
+  const int per_cta = a.per_seg ? 0 : (N + gridDim.x - 1) / gridDim.x;
+  if (blockIdx.x == 0 && a.header)
+    for (int i = tid; i < a.B + 2; i += kWarps * 32) a.header[i] = i ? prefix[i - 1] : per_cta;
+
+  // sequences without a position
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+    if (prefix[b + 1] == prefix[b])
+      for (int i = tid; i < a.H * (kHeadDim / 8); i += kWarps * 32)
+        reinterpret_cast<uint4*>(a.o + (long)b * a.ldo)[i] = make_uint4(0, 0, 0, 0);
+
+  // this CTA's run of the list, and this warp's
+  int R0, R1;
+  if (a.per_seg) {
+    const int b = blockIdx.x / Hc, T = prefix[b + 1] - prefix[b];
+    R0 = prefix[b] * Hc + (blockIdx.x % Hc) * T;
+    R1 = R0 + T;
+  } else {
+    R0 = min(N, (int)blockIdx.x * per_cta);
+    R1 = min(N, R0 + per_cta);
+  }
+  const int pw = (R1 - R0 + kWarps - 1) / kWarps;
+  const int beg = min(R1, R0 + warp * pw), end = min(R1, beg + pw);
+
+  if (beg < end) {
+    Place at = place_of(prefix, a.B, Hc, beg);
+    int win = beg, pg0 = 0, pg1 = 0, row0 = 0, row1 = 0;      // coordinates of tile win + lane
+    auto look_up = [&](int first) {
+      win = first;
+      if (first + lane < end) {
+        const Place p = place_of(prefix, a.B, Hc, first + lane);
+        const int pos = p.t * kTile, seq = seq_of(a, p.b), kh = p.hc / a.chunks;
+        const int* tab = a.c.table + (long)p.b * a.c.ld_table;
+        pg0 = tab[pos / a.c.page];
+        row0 = kh * a.c.page + pos % a.c.page;
+        bool bad = pg0 < 0 || pg0 >= a.c.n_pages;
+        if (bad) pg0 = a.c.n_pages;
+        if (a.two_boxes) {
+          const int p1 = pos + kTile / 2;
+          pg1 = a.c.n_pages;
+          if (p1 < seq) {
+            pg1 = tab[p1 / a.c.page];
+            if (pg1 < 0 || pg1 >= a.c.n_pages) pg1 = a.c.n_pages, bad = true;
+          }
+          row1 = kh * a.c.page + p1 % a.c.page;
+        }
+        if (bad) atomicOr(&g_attn_status, kPagedBadPage);
+      }
+    };
+    auto issue = [&](int x, int slot) {                       // whole warp; x < end
+      if (x >= win + 32) look_up(x);
+      const int s = x - win;
+      const int p0 = __shfl_sync(0xffffffffu, pg0, s), r0 = __shfl_sync(0xffffffffu, row0, s);
+      const int p1 = __shfl_sync(0xffffffffu, pg1, s), r1 = __shfl_sync(0xffffffffu, row1, s);
+      if (lane == 0) {
+        const uint32_t k = smem_u32(ring + slot * 2 * kTileBytes), v = k + kTileBytes;
+        mbar_expect_tx(&wbars[slot], 2 * kTileBytes);
+        load_box(k, &tmk, r0, p0, &wbars[slot]);
+        load_box(v, &tmv, r0, p0, &wbars[slot]);
+        if (a.two_boxes) {
+          load_box(k + kTileBytes / 2, &tmk, r1, p1, &wbars[slot]);
+          load_box(v + kTileBytes / 2, &tmv, r1, p1, &wbars[slot]);
+        }
+      }
+    };
+    look_up(beg);
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s)
+      if (beg + s < end) issue(beg + s, s);
+
+    uint32_t qa[8], qb[8];
+    float m = -1e30f, l = 0.f, scale = 0.f, oacc[16][4];
+    int seq = 0;
+    bool first = at.t == 0;                                   // the segment began in this warp
+    auto start_segment = [&]() {
+      const int kh = at.hc / a.chunks, head = (at.hc % a.chunks) * kGroup + g;
+      seq = seq_of(a, at.b);
+      scale = (a.c.k_scale ? a.c.k_scale[kh] : 1.f) * rsqrtf((float)kHeadDim) * 1.4426950408889634f;
+      const uint4* qp = reinterpret_cast<const uint4*>(a.q + (long)at.b * a.ldq +
+                                                       ((long)kh * a.Hg + head) * kHeadDim + 32 * t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint4 v = head < a.Hg ? qp[i] : make_uint4(0, 0, 0, 0);
+        qa[2 * i] = v.x; qb[2 * i] = v.y; qa[2 * i + 1] = v.z; qb[2 * i + 1] = v.w;
+      }
+      m = -1e30f;
+      l = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) oacc[j][i] = 0.f;
+    };
+    start_segment();
+
+    int slot = 0;
+    unsigned parity = 0;
+    for (int x = beg; x < end; ++x) {
+      if (!wait_full(&wbars[slot], parity)) {                 // drain what is in flight and stop
+        if (lane == 0) atomicOr(&g_attn_status, kPagedTimeout);
+        for (int y = x + 1; y < min(end, x + kSlots); ++y) {
+          slot = slot + 1 == kSlots ? 0 : slot + 1;
+          if (slot == 0) parity ^= 1;
+          wait_full(&wbars[slot], parity);
+        }
+        break;
+      }
+      const uint32_t kb = smem_u32(ring + slot * 2 * kTileBytes), vb = kb + kTileBytes;
+      const int nvalid = min(kTile, seq - at.t * kTile);
+      if (nvalid < kTile) {                                   // rows behind the sequence may hold anything
+        for (int i = lane; i < (kTile - nvalid) * 8; i += 32)
+          reinterpret_cast<uint4*>(ring + slot * 2 * kTileBytes + kTileBytes)[nvalid * 8 + i] = make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the slot's next load comes after these writes
+        __syncwarp();
+      }
+      // ---- S = Q K^T, 4 x 8 positions
+      float sc[4][2];
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) {
+        const int pr = nt * 8 + g;
+        const uint4 k0 = lds128(kb + pr * 128 + (((2 * t) ^ (pr & 7)) << 4));
+        const uint4 k1 = lds128(kb + pr * 128 + (((2 * t + 1) ^ (pr & 7)) << 4));
+        const uint32_t kw[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          mma16816(c, qa[j], 0u, qb[j], 0u, fp8x2_to_h2((uint16_t)(kw[j] & 0xFFFFu)),
+                   fp8x2_to_h2((uint16_t)(kw[j] >> 16)));
+        const int p0 = nt * 8 + 2 * t;
+        sc[nt][0] = p0 < nvalid ? c[0] * scale : -INFINITY;
+        sc[nt][1] = p0 + 1 < nvalid ? c[1] * scale : -INFINITY;
+      }
+      // ---- running maximum and weights
+      float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1])),
+                       fmaxf(fmaxf(sc[2][0], sc[2][1]), fmaxf(sc[3][0], sc[3][1])));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      if (__any_sync(0xffffffffu, mx > m)) {
+        const float mn = fmaxf(m, mx), f = ex2(m - mn);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) oacc[j][i] *= f;
+      }
+      uint32_t ph[4], pl[4];                                  // rounded weights and remainders
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt) {
+        const float e0 = ex2(sc[nt][0] - m), e1 = ex2(sc[nt][1] - m);
+        l += e0 + e1;
+        const __half2 h = __floats2half2_rn(e0, e1);
+        const float2 r = __half22float2(h);
+        ph[nt] = h2_as_u32(h);
+        pl[nt] = h2_as_u32(__floats2half2_rn(e0 - r.x, e1 - r.y));
+      }
+      // ---- O += P V, 2 x 16 positions
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        const int r0 = kk * 16 + 2 * t, r1 = r0 + 1, r2 = r0 + 8, r3 = r0 + 9;
+        const uint4 v0 = lds128(vb + r0 * 128 + ((g ^ (r0 & 7)) << 4));
+        const uint4 v1 = lds128(vb + r1 * 128 + ((g ^ (r1 & 7)) << 4));
+        const uint4 v2 = lds128(vb + r2 * 128 + ((g ^ (r2 & 7)) << 4));
+        const uint4 v3 = lds128(vb + r3 * 128 + ((g ^ (r3 & 7)) << 4));
+        const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
+        const uint32_t w2[4] = {v2.x, v2.y, v2.z, v2.w}, w3[4] = {v3.x, v3.y, v3.z, v3.w};
+#pragma unroll
+        for (int wi = 0; wi < 4; ++wi) {
+          // bytes of rows (r0, r1) and (r2, r3) side by side
+          const uint32_t lo01 = prmt(w0[wi], w1[wi], 0x5140u), hi01 = prmt(w0[wi], w1[wi], 0x7362u);
+          const uint32_t lo23 = prmt(w2[wi], w3[wi], 0x5140u), hi23 = prmt(w2[wi], w3[wi], 0x7362u);
+          const uint32_t p01[4] = {lo01 & 0xFFFFu, lo01 >> 16, hi01 & 0xFFFFu, hi01 >> 16};
+          const uint32_t p23[4] = {lo23 & 0xFFFFu, lo23 >> 16, hi23 & 0xFFFFu, hi23 >> 16};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)                         // element 16 g + 4 wi + k of the head
+            mma16816(oacc[4 * wi + k], ph[2 * kk], pl[2 * kk], ph[2 * kk + 1], pl[2 * kk + 1],
+                     fp8x2_to_h2((uint16_t)p01[k]), fp8x2_to_h2((uint16_t)p23[k]));
+        }
+      }
+      __syncwarp();                                           // the slot is read; the next load may overwrite it
+      if (x + kSlots < end) {
+        if (lane == 0) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        issue(x + kSlots, slot);
+      }
+      slot = slot + 1 == kSlots ? 0 : slot + 1;
+      if (slot == 0) parity ^= 1;
+
+      // ---- end of the segment, or of this warp's run
+      const bool last = at.t + 1 == at.T;
+      if (last || x + 1 == end) {
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        const int kh = at.hc / a.chunks, hg = (at.hc % a.chunks) * kGroup + g;
+        if (first && last) {                                  // whole: lane holds elements 32 t .. 32 t + 31 of head g
+          float v[32];
+          const float inv = l > 0.f ? (a.c.v_scale ? a.c.v_scale[kh] : 1.f) / l : 0.f;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            v[j] = (oacc[j][0] + oacc[j][2]) * inv;
+            v[16 + j] = (oacc[j][1] + oacc[j][3]) * inv;
+          }
+          if (a.fwht) fwht32_regs(v);
+          if (hg < a.Hg) {
+            uint4* dst = reinterpret_cast<uint4*>(a.o + (long)at.b * a.ldo + ((long)kh * a.Hg + hg) * kHeadDim + 32 * t);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              dst[i] = make_uint4(h2_as_u32(__floats2half2_rn(v[8 * i], v[8 * i + 1])),
+                                  h2_as_u32(__floats2half2_rn(v[8 * i + 2], v[8 * i + 3])),
+                                  h2_as_u32(__floats2half2_rn(v[8 * i + 4], v[8 * i + 5])),
+                                  h2_as_u32(__floats2half2_rn(v[8 * i + 6], v[8 * i + 7])));
+          }
+        } else {
+          const int which = last ? 0 : 1;                     // head: ends here; tail: goes on in the next warp
+          float* p = part0 + (2 * warp + which) * kPartFloats + g * kPitch;
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            *reinterpret_cast<float4*>(p + 32 * t + j) =
+                make_float4(oacc[j][0] + oacc[j][2], oacc[j + 1][0] + oacc[j + 1][2], oacc[j + 2][0] + oacc[j + 2][2],
+                            oacc[j + 3][0] + oacc[j + 3][2]);
+            *reinterpret_cast<float4*>(p + 32 * t + 16 + j) =
+                make_float4(oacc[j][1] + oacc[j][3], oacc[j + 1][1] + oacc[j + 1][3], oacc[j + 2][1] + oacc[j + 2][3],
+                            oacc[j + 3][1] + oacc[j + 3][3]);
+          }
+          if (t == 0) {
+            p[kHeadDim] = m;
+            p[kHeadDim + 1] = l;
+          }
+          if (lane == 0) meta[2 * warp + which] = at.b * Hc + at.hc;
+        }
+        if (x + 1 < end) {                                    // the next segment
+          at.t = 0;
+          if (++at.hc == Hc) {
+            at.hc = 0;
+            do { ++at.b; } while (prefix[at.b + 1] == prefix[at.b]);
+            at.T = prefix[at.b + 1] - prefix[at.b];
+          }
+          first = true;
+          start_segment();
+        }
+      } else {
+        ++at.t;
+      }
+    }
+  }
+  __syncthreads();
+
+  // ---- join the parts of this CTA, segment by segment; a warp per head
+  for (int w = 0; w < kWarps; ++w)
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      const int seg = meta[2 * w + which];
+      if (seg < 0) continue;
+      // its first part here: a head only in the first warp, a tail that does not go on from the warp before
+      if (which == 0 ? w > 0 : w > 0 && meta[2 * w - 1] == seg) continue;
+      int n = 1;                                              // parts: tails of w, w + 1, .. and the closing head
+      if (which == 1)
+        for (int u = w + 1; u < kWarps; ++u) {
+          if (meta[2 * u] != seg && meta[2 * u + 1] != seg) break;
+          ++n;
+          if (meta[2 * u] == seg) break;
+        }
+      const int b = seg / Hc, hc = seg % Hc, T = prefix[b + 1] - prefix[b], s0 = prefix[b] * Hc + hc * T;
+      const int kh = hc / a.chunks, hg = (hc % a.chunks) * kGroup + warp;
+      if (hg >= a.Hg) continue;
+      float M, L, O[4];
+      join(n, lane, [&](int i) {
+        const int u = w + i;
+        return part0 + (2 * u + (meta[2 * u] == seg ? 0 : 1)) * kPartFloats + warp * kPitch;
+      }, M, L, O);
+      if (s0 >= R0 && s0 + T <= R1) {
+        store_head(a, b, kh * a.Hg + hg, kh, L, O, lane);
+      } else {
+        float* p = a.parts + ((long)blockIdx.x * 2 + (s0 < R0 ? 0 : 1)) * kPartFloats + warp * kPitch;
+        *reinterpret_cast<float4*>(p + 4 * lane) = make_float4(O[0], O[1], O[2], O[3]);
+        if (lane == 0) {
+          p[kHeadDim] = M;
+          p[kHeadDim + 1] = L;
+        }
+      }
+    }
+}
+
+// Joins the (sequence, head) parts that lie in several CTAs: a CTA per (sequence, kv head, group), a warp per head.
+__global__ void __launch_bounds__(kGroup * 32) paged_join_kernel(const AttnArgs a) {
+  pdl_wait_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, Hc = a.c.Hk * a.chunks;
+  const int b = blockIdx.x / Hc, hc = blockIdx.x % Hc, kh = hc / a.chunks, hg = (hc % a.chunks) * kGroup + warp;
+  const int per_cta = a.header[0], p0 = a.header[1 + b], T = a.header[2 + b] - p0;
+  if (T == 0 || hg >= a.Hg) return;
+  const int s0 = p0 * Hc + hc * T, c0 = s0 / per_cta, c1 = (s0 + T - 1) / per_cta;
+  if (c0 == c1) return;
+  float M, L, O[4];
+  join(c1 - c0 + 1, lane, [&](int i) {
+    return a.parts + ((long)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats + warp * kPitch;
+  }, M, L, O);
+  store_head(a, b, kh * a.Hg + hg, kh, L, O, lane);
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+int page_map(CUtensorMap* m, const void* base, const PagedView& c, long stride, int rows) {
+  static EncodeTiled fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiled>(f);
+  });
+  if (!fn) return set_error(R4Q_ERR_CUDA, "paged_flash_decode: cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[3] = {(cuuint64_t)kHeadDim, (cuuint64_t)c.Hk * c.page, (cuuint64_t)c.n_pages};
+  cuuint64_t strides[2] = {(cuuint64_t)kHeadDim, (cuuint64_t)stride};
+  cuuint32_t box[3] = {(cuuint32_t)kHeadDim, (cuuint32_t)rows, 1};
+  cuuint32_t es[3] = {1, 1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(R4Q_ERR_CUDA, "paged_flash_decode: tensor map encode failed (%d)", (int)r);
+  return R4Q_OK;
+}
+
+size_t smem_bytes(int B) {
+  return 1024 + (size_t)kWarps * kSlots * 2 * kTileBytes + (size_t)kWarps * 2 * kPartFloats * 4 +
+         kWarps * kSlots * 8 + 3 * kWarps * 4 + (size_t)(B + 1) * 4;
+}
+
+// Sequences whose table holds so few positions that a CTA per (sequence, head)
+// gives a warp two tiles at most are not split: no second kernel.
+bool per_segment(int page, int max_blocks) { return (long)max_blocks * page <= 2L * kWarps * kTile; }
+
+int grid_ctas() { return num_sms(); }
+
+size_t header_bytes(int B) { return ((size_t)(B + 2) * 4 + 15) / 16 * 16; }
 
 }  // namespace
 
@@ -78,19 +556,21 @@ cudaError_t paged_attn_status(int clear, int* word) {
 using namespace r4q;
 
 extern "C" size_t r4q_paged_flash_decode_workspace_bytes(int B, int H, int Hk, int page, int max_blocks) {
-  (void)B; (void)H; (void)Hk; (void)page; (void)max_blocks;
-  return 0;
+  if (B < 1 || H < 1 || Hk < 1 || page < 1 || max_blocks < 1 || per_segment(page, max_blocks)) return 0;
+  return header_bytes(B) + (size_t)grid_ctas() * 2 * kPartFloats * 4;
 }
 
 extern "C" int r4q_paged_flash_decode(const void* q, long ldq, const r4q_paged_cache* cache,
                                       const long long* seq_lens, void* o, long ldo, int B, int H, int flags,
                                       void* workspace, size_t ws_bytes, void* stream) {
-  PagedView c;
-  int st = paged_view("paged_flash_decode", cache, &c);
+  AttnArgs a{};
+  int st = paged_view("paged_flash_decode", cache, &a.c);
   if (st) return st;
-  if (B < 0 || B > 4096 || B > c.seqs)
-    return set_error(R4Q_ERR_ARG, "paged_flash_decode: batch %d (at most 4096 and the table's %d rows)", B, c.seqs);
-  if (H < c.Hk || H % c.Hk || H > 65535) return set_error(R4Q_ERR_ARG, "paged_flash_decode: bad heads H=%d Hk=%d", H, c.Hk);
+  if (B < 0 || B > kMaxBatch || B > a.c.seqs)
+    return set_error(R4Q_ERR_ARG, "paged_flash_decode: batch %d (at most %d and the table's %d rows)", B, kMaxBatch,
+                     a.c.seqs);
+  if (H < a.c.Hk || H % a.c.Hk || H > 65535)
+    return set_error(R4Q_ERR_ARG, "paged_flash_decode: bad heads H=%d Hk=%d", H, a.c.Hk);
   if (flags & ~R4Q_ATTN_FWHT) return set_error(R4Q_ERR_ARG, "paged_flash_decode: unknown flags %d", flags);
   if (B == 0) return R4Q_OK;
   if (!q || !o || !seq_lens) return set_error(R4Q_ERR_ARG, "paged_flash_decode: null pointer");
@@ -98,10 +578,56 @@ extern "C" int r4q_paged_flash_decode(const void* q, long ldq, const r4q_paged_c
     return set_error(R4Q_ERR_ARG, "paged_flash_decode: row strides below H * 128");
   if (!aligned(q, 16) || (B > 1 && ldq % 8) || !aligned(o, 16) || (B > 1 && ldo % 8))
     return set_error(R4Q_ERR_ALIGN, "paged_flash_decode: q and o must be 16-byte aligned, strides multiples of 8");
-  const size_t need = r4q_paged_flash_decode_workspace_bytes(B, H, c.Hk, c.page, c.max_blocks);
+  a.Hg = H / a.c.Hk;
+  a.chunks = (a.Hg + kGroup - 1) / kGroup;
+  const int Hc = a.c.Hk * a.chunks;
+  const long cap = (long)a.c.max_blocks * a.c.page;
+  if ((cap / kTile + 1) * B * Hc > 0x7fffffffL - 65536)
+    return set_error(R4Q_ERR_ARG, "paged_flash_decode: %d sequences of %ld positions and %d heads are too many tiles",
+                     B, cap, Hc);
+  a.per_seg = per_segment(a.c.page, a.c.max_blocks);
+  const size_t need = a.per_seg ? 0 : r4q_paged_flash_decode_workspace_bytes(B, H, a.c.Hk, a.c.page, a.c.max_blocks);
   if (need && (!workspace || ws_bytes < need))
     return set_error(R4Q_ERR_CAPACITY, "paged_flash_decode: workspace %zu < %zu bytes", ws_bytes, need);
-  paged_attn_kernel<<<dim3(H, B), kWarps * 32, 0, (cudaStream_t)stream>>>(
-      (const __half*)q, ldq, c, seq_lens, (__half*)o, ldo, H / c.Hk, flags & R4Q_ATTN_FWHT);
-  return check_launch("paged_attn_kernel");
+  if (need && !aligned(workspace, 16)) return set_error(R4Q_ERR_ALIGN, "paged_flash_decode: workspace misaligned");
+  a.q = (const __half*)q; a.ldq = ldq;
+  a.seq_lens = seq_lens;
+  a.o = (__half*)o; a.ldo = ldo;
+  a.B = B; a.H = H; a.fwht = (flags & R4Q_ATTN_FWHT) ? 1 : 0;
+  a.two_boxes = a.c.page % kTile != 0;
+  if (need) {
+    a.header = (int*)workspace;
+    a.parts = (float*)((uint8_t*)workspace + header_bytes(B));
+  }
+  CUtensorMap tmk, tmv;
+  const int rows = a.two_boxes ? kTile / 2 : kTile;
+  st = page_map(&tmk, a.c.k, a.c, a.c.k_stride, rows);
+  if (!st) st = page_map(&tmv, a.c.v, a.c, a.c.v_stride, rows);
+  if (st) return st;
+  static std::mutex mu;
+  static bool attr_done[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (dev >= 64 || !attr_done[dev]) {
+      const cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)smem_bytes(kMaxBatch));
+      if (e != cudaSuccess) {
+        cudaGetLastError();
+        return set_error(R4Q_ERR_CUDA, "paged_attn_kernel: %s", cudaGetErrorString(e));
+      }
+      if (dev < 64) attr_done[dev] = true;
+    }
+  }
+  cudaStream_t s = (cudaStream_t)stream;
+  const unsigned ctas = a.per_seg ? (unsigned)(B * Hc) : (unsigned)grid_ctas();
+  cudaError_t e = launch_pdl(paged_attn_kernel, dim3(ctas), dim3(kWarps * 32), smem_bytes(B), s, tmk, tmv, a);
+  if (e == cudaSuccess && !a.per_seg)
+    e = launch_pdl(paged_join_kernel, dim3((unsigned)(B * Hc)), dim3((unsigned)(min(a.Hg, kGroup) * 32)), 0, s, a);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(R4Q_ERR_CUDA, "paged_attn_kernel: %s", cudaGetErrorString(e));
+  }
+  return R4Q_OK;
 }
