@@ -51,8 +51,22 @@ constexpr int kTileBytes = kTile * kHeadDim;      // of K, and of V
 constexpr int kGroup = 8;                         // query heads per pass over K and V
 constexpr int kPitch = 132;                       // floats of a part's head: O[128], m, l, padding
 constexpr int kPartFloats = kGroup * kPitch;
-constexpr int kMaxBatch = 4096;
+constexpr int kMaxBatch = 2048;
+constexpr int kJoinWarps = 4;
 constexpr int kWaitPolls = 1 << 22;
+
+// x / d for 0 <= x < 2^31 by a multiplication: m = ceil(2^(31 + s) / d), 2^(s-1) < d <= 2^s
+// (Granlund and Montgomery, Division by invariant integers using multiplication, 1994)
+struct FastDiv {
+  uint32_t m;
+  int s;
+  __device__ __forceinline__ int div(int x) const { return (int)(((uint64_t)m * (uint32_t)x) >> (31 + s)); }
+};
+FastDiv fast_div(uint32_t d) {
+  int s = 0;
+  while ((1ull << s) < d) ++s;
+  return FastDiv{(uint32_t)(((1ull << (31 + s)) + d - 1) / d), s};
+}
 
 struct AttnArgs {
   const __half* q;
@@ -61,7 +75,8 @@ struct AttnArgs {
   const long long* seq_lens;
   __half* o;
   long ldo;
-  int B, H, Hg, chunks, fwht;
+  int B, H, Hg, Hc, chunks, fwht;  // Hc: kv heads x groups of 8 query heads
+  FastDiv by_page, by_Hc, by_chunks;
   int per_seg;       // a CTA per (sequence, head, group) instead of equal runs
   int two_boxes;     // 16-position boxes
   int* header;       // workspace: tiles per CTA, then the prefix sums of tiles [B + 1]
@@ -105,25 +120,45 @@ __device__ __forceinline__ void fwht32_x4(float (&v)[4], int lane) {
   for (int i = 0; i < 4; ++i) v[i] *= kInvSqrt32;
 }
 
-// A warp joins n parts of one head (part(i): its 132 floats) and gives O, unnormalised, 4 per lane.
-template <typename F>
-__device__ __forceinline__ void join(int n, int lane, F part, float& M, float& L, float (&O)[4]) {
-  M = -1e30f;
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, part(i)[kHeadDim]);
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
-  L = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) O[i] = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const float* p = part(i);
-    const float f = ex2(p[kHeadDim] - M);
-    const float4 v = *reinterpret_cast<const float4*>(p + 4 * lane);
-    L += p[kHeadDim + 1] * f;
-    O[0] += v.x * f; O[1] += v.y * f; O[2] += v.z * f; O[3] += v.w * f;
+// The running join of parts of a head, O 4 elements per lane.
+struct Joined {
+  float M = -1e30f, L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(float m, float l, const float4 v) {
+    const float mn = fmaxf(M, m), f = ex2(M - mn), e = ex2(m - mn);
+    M = mn;
+    L = L * f + l * e;
+    O[0] = O[0] * f + v.x * e;
+    O[1] = O[1] * f + v.y * e;
+    O[2] = O[2] * f + v.z * e;
+    O[3] = O[3] * f + v.w * e;
   }
-}
+  // parts i = first, first + step, .. < n at part(i): the loads of four go out together
+  template <typename F>
+  __device__ __forceinline__ void add_all(int first, int step, int n, int lane, F part) {
+    for (int i = first; i < n; i += 4 * step) {
+      float4 v[4];
+      float m[4], l[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j * step < n) {
+          const float* p = part(i + j * step);
+          v[j] = *reinterpret_cast<const float4*>(p + 4 * lane);
+          m[j] = p[kHeadDim];
+          l[j] = p[kHeadDim + 1];
+        }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j * step < n) add(m[j], l[j], v[j]);
+    }
+  }
+  __device__ __forceinline__ void put(float* p, int lane) const {
+    *reinterpret_cast<float4*>(p + 4 * lane) = make_float4(O[0], O[1], O[2], O[3]);
+    if (lane == 0) {
+      p[kHeadDim] = M;
+      p[kHeadDim + 1] = L;
+    }
+  }
+};
 __device__ __forceinline__ void store_head(const AttnArgs& a, int b, int head, int kh, float L, float (&O)[4],
                                            int lane) {
   const float inv = L > 0.f ? (a.c.v_scale ? a.c.v_scale[kh] : 1.f) / L : 0.f;
@@ -134,23 +169,18 @@ __device__ __forceinline__ void store_head(const AttnArgs& a, int b, int head, i
       make_uint2(h2_as_u32(__floats2half2_rn(O[0], O[1])), h2_as_u32(__floats2half2_rn(O[2], O[3])));
 }
 
-__device__ __forceinline__ int seq_of(const AttnArgs& a, int b) {
-  const long long s = a.seq_lens[b], cap = (long long)a.c.max_blocks * a.c.page;
-  return (int)(s < 0 ? 0 : s > cap ? cap : s);
-}
-
 struct Place {                 // of a tile in the list
   int b, hc, t, T;             // sequence, kv head * chunks + chunk, tile and tiles of the sequence
 };
-__device__ __forceinline__ Place place_of(const int* prefix, int B, int Hc, int x) {
-  const int y = x / Hc;
-  int lo = 0, hi = B;                               // prefix[lo] <= y < prefix[hi]
+__device__ __forceinline__ Place place_of(const int* prefix, const AttnArgs& a, int x) {
+  const int y = a.by_Hc.div(x);
+  int lo = 0, hi = a.B;                               // prefix[lo] <= y < prefix[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (prefix[mid] <= y) lo = mid; else hi = mid;
   }
-  const int T = prefix[lo + 1] - prefix[lo], rem = x - prefix[lo] * Hc;
-  return Place{lo, rem / T, rem % T, T};
+  const int T = prefix[lo + 1] - prefix[lo], rem = x - prefix[lo] * a.Hc, hc = rem / T;
+  return Place{lo, hc, rem - hc * T, T};
 }
 
 __global__ void __launch_bounds__(kWarps * 32, 1)
@@ -164,28 +194,35 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(part0 + kWarps * 2 * kPartFloats);
   int* meta = reinterpret_cast<int*>(bars + kWarps * kSlots);                          // [warp][head, tail] segment
   int* wsum = meta + 2 * kWarps;
-  int* prefix = wsum + kWarps;                                                        // [B + 1]
+  int* prefix = wsum + kWarps;                                                        // [B + 1] tiles before
+  int* seqs = prefix + a.B + 1;                                                       // [B] lengths
   uint64_t* wbars = bars + warp * kSlots;
-  const int Hc = a.c.Hk * a.chunks;
+  const int Hc = a.Hc;
 
   if (lane == 0) {
     for (int s = 0; s < kSlots; ++s) mbar_init(&wbars[s], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     meta[2 * warp] = meta[2 * warp + 1] = -1;
   }
+  if (tid == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmk)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmv)) : "memory");
+  }
   pdl_wait_trigger();
 
-  // prefix sums of the tiles of the sequences
+  // lengths, and the prefix sums of their tiles
   {
     const int each = (a.B + kWarps * 32 - 1) / (kWarps * 32), b0 = tid * each;
+    const long long cap = (long long)a.c.max_blocks * a.c.page;
     int own = 0;
     bool bad = false;
-    for (int i = 0; i < each; ++i)
-      if (b0 + i < a.B) {
-        const int n = seq_of(a, b0 + i);
-        bad |= n != a.seq_lens[b0 + i];
-        own += (n + kTile - 1) / kTile;
-      }
+    for (int b = b0; b < min(a.B, b0 + each); ++b) {
+      const long long n = a.seq_lens[b];
+      bad |= n < 0 || n > cap;
+      const int len = (int)(n < 0 ? 0 : n > cap ? cap : n);
+      seqs[b] = len;
+      own += (len + kTile - 1) / kTile;
+    }
     if (bad && blockIdx.x == 0) atomicOr(&g_attn_status, kPagedBadPage);
     int inc = own;
 #pragma unroll
@@ -196,31 +233,28 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     if (lane == 31) wsum[warp] = inc;
     __syncthreads();
     int at = inc - own;
-    for (int w = 0; w < warp; ++w) at += wsum[w];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) at += w < warp ? wsum[w] : 0;
     if (tid == 0) prefix[0] = 0;
-    for (int i = 0; i < each; ++i)
-      if (b0 + i < a.B) {
-        at += (seq_of(a, b0 + i) + kTile - 1) / kTile;
-        prefix[b0 + i + 1] = at;
-      }
+    for (int b = b0; b < min(a.B, b0 + each); ++b) prefix[b + 1] = at += (seqs[b] + kTile - 1) / kTile;
     __syncthreads();
   }
   const int N = prefix[a.B] * Hc;
-  const int per_cta = a.per_seg ? 0 : (N + gridDim.x - 1) / gridDim.x;
+  // at least a tile per warp: fewer parts to join
+  const int per_cta = a.per_seg ? 0 : max(kWarps, (N + (int)gridDim.x - 1) / (int)gridDim.x);
   if (blockIdx.x == 0 && a.header)
     for (int i = tid; i < a.B + 2; i += kWarps * 32) a.header[i] = i ? prefix[i - 1] : per_cta;
 
-  // sequences without a position
   for (int b = blockIdx.x; b < a.B; b += gridDim.x)
-    if (prefix[b + 1] == prefix[b])
+    if (prefix[b + 1] == prefix[b])                           // a sequence without a position
       for (int i = tid; i < a.H * (kHeadDim / 8); i += kWarps * 32)
         reinterpret_cast<uint4*>(a.o + (long)b * a.ldo)[i] = make_uint4(0, 0, 0, 0);
 
   // this CTA's run of the list, and this warp's
   int R0, R1;
   if (a.per_seg) {
-    const int b = blockIdx.x / Hc, T = prefix[b + 1] - prefix[b];
-    R0 = prefix[b] * Hc + (blockIdx.x % Hc) * T;
+    const int b = a.by_Hc.div(blockIdx.x), T = prefix[b + 1] - prefix[b];
+    R0 = prefix[b] * Hc + ((int)blockIdx.x - b * Hc) * T;
     R1 = R0 + T;
   } else {
     R0 = min(N, (int)blockIdx.x * per_cta);
@@ -230,27 +264,24 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   const int beg = min(R1, R0 + warp * pw), end = min(R1, beg + pw);
 
   if (beg < end) {
-    Place at = place_of(prefix, a.B, Hc, beg);
+    Place at = place_of(prefix, a, beg);
     int win = beg, pg0 = 0, pg1 = 0, row0 = 0, row1 = 0;      // coordinates of tile win + lane
     auto look_up = [&](int first) {
       win = first;
       if (first + lane < end) {
-        const Place p = place_of(prefix, a.B, Hc, first + lane);
-        const int pos = p.t * kTile, seq = seq_of(a, p.b), kh = p.hc / a.chunks;
+        const Place p = place_of(prefix, a, first + lane);
+        const int pos = p.t * kTile, kh = a.by_chunks.div(p.hc), blk = a.by_page.div(pos);
         const int* tab = a.c.table + (long)p.b * a.c.ld_table;
-        pg0 = tab[pos / a.c.page];
-        row0 = kh * a.c.page + pos % a.c.page;
-        bool bad = pg0 < 0 || pg0 >= a.c.n_pages;
-        if (bad) pg0 = a.c.n_pages;
+        pg0 = tab[blk];
+        row0 = (kh - blk) * a.c.page + pos;
+        bool bad = false;
         if (a.two_boxes) {
-          const int p1 = pos + kTile / 2;
-          pg1 = a.c.n_pages;
-          if (p1 < seq) {
-            pg1 = tab[p1 / a.c.page];
-            if (pg1 < 0 || pg1 >= a.c.n_pages) pg1 = a.c.n_pages, bad = true;
-          }
-          row1 = kh * a.c.page + p1 % a.c.page;
+          const int p1 = pos + kTile / 2, blk1 = a.by_page.div(p1);
+          pg1 = p1 < seqs[p.b] ? tab[blk1] : 0;
+          row1 = (kh - blk1) * a.c.page + p1;
+          if (pg1 < 0 || pg1 >= a.c.n_pages) pg1 = a.c.n_pages, bad = true;
         }
+        if (pg0 < 0 || pg0 >= a.c.n_pages) pg0 = a.c.n_pages, bad = true;
         if (bad) atomicOr(&g_attn_status, kPagedBadPage);
       }
     };
@@ -270,18 +301,13 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
         }
       }
     };
-    look_up(beg);
-#pragma unroll
-    for (int s = 0; s < kSlots; ++s)
-      if (beg + s < end) issue(beg + s, s);
-
     uint32_t qa[8], qb[8];
     float m = -1e30f, l = 0.f, scale = 0.f, oacc[16][4];
     int seq = 0;
     bool first = at.t == 0;                                   // the segment began in this warp
     auto start_segment = [&]() {
-      const int kh = at.hc / a.chunks, head = (at.hc % a.chunks) * kGroup + g;
-      seq = seq_of(a, at.b);
+      const int kh = a.by_chunks.div(at.hc), head = (at.hc - kh * a.chunks) * kGroup + g;
+      seq = seqs[at.b];
       scale = (a.c.k_scale ? a.c.k_scale[kh] : 1.f) * rsqrtf((float)kHeadDim) * 1.4426950408889634f;
       const uint4* qp = reinterpret_cast<const uint4*>(a.q + (long)at.b * a.ldq +
                                                        ((long)kh * a.Hg + head) * kHeadDim + 32 * t);
@@ -298,6 +324,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
         for (int i = 0; i < 4; ++i) oacc[j][i] = 0.f;
     };
     start_segment();
+
+    look_up(beg);
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s)
+      if (beg + s < end) issue(beg + s, s);
 
     int slot = 0;
     unsigned parity = 0;
@@ -396,7 +427,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       if (last || x + 1 == end) {
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-        const int kh = at.hc / a.chunks, hg = (at.hc % a.chunks) * kGroup + g;
+        const int kh = a.by_chunks.div(at.hc), hg = (at.hc - kh * a.chunks) * kGroup + g;
         if (first && last) {                                  // whole: lane holds elements 32 t .. 32 t + 31 of head g
           float v[32];
           const float inv = l > 0.f ? (a.c.v_scale ? a.c.v_scale[kh] : 1.f) / l : 0.f;
@@ -451,55 +482,64 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   __syncthreads();
 
   // ---- join the parts of this CTA, segment by segment; a warp per head
-  for (int w = 0; w < kWarps; ++w)
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const int seg = meta[2 * w + which];
-      if (seg < 0) continue;
-      // its first part here: a head only in the first warp, a tail that does not go on from the warp before
-      if (which == 0 ? w > 0 : w > 0 && meta[2 * w - 1] == seg) continue;
-      int n = 1;                                              // parts: tails of w, w + 1, .. and the closing head
-      if (which == 1)
+  // Lane 2 w + which looks at part (w, which): it opens a segment of this CTA if it
+  // is the head of the first warp, or a tail that does not go on from the warp
+  // before; then come the tails of the next warps, up to the head that closes it.
+  unsigned open = 0;
+  int mine = -1, parts = 0;
+  if (lane < 2 * kWarps) {
+    const int w = lane >> 1;
+    mine = meta[lane];
+    if (mine >= 0 && (lane & 1 ? w == 0 || meta[lane - 2] != mine : w == 0)) {
+      parts = 1;
+      if (lane & 1)
         for (int u = w + 1; u < kWarps; ++u) {
-          if (meta[2 * u] != seg && meta[2 * u + 1] != seg) break;
-          ++n;
-          if (meta[2 * u] == seg) break;
+          const int h = meta[2 * u];
+          if (h != mine && meta[2 * u + 1] != mine) break;
+          ++parts;
+          if (h == mine) break;
         }
-      const int b = seg / Hc, hc = seg % Hc, T = prefix[b + 1] - prefix[b], s0 = prefix[b] * Hc + hc * T;
-      const int kh = hc / a.chunks, hg = (hc % a.chunks) * kGroup + warp;
-      if (hg >= a.Hg) continue;
-      float M, L, O[4];
-      join(n, lane, [&](int i) {
-        const int u = w + i;
-        return part0 + (2 * u + (meta[2 * u] == seg ? 0 : 1)) * kPartFloats + warp * kPitch;
-      }, M, L, O);
-      if (s0 >= R0 && s0 + T <= R1) {
-        store_head(a, b, kh * a.Hg + hg, kh, L, O, lane);
-      } else {
-        float* p = a.parts + ((long)blockIdx.x * 2 + (s0 < R0 ? 0 : 1)) * kPartFloats + warp * kPitch;
-        *reinterpret_cast<float4*>(p + 4 * lane) = make_float4(O[0], O[1], O[2], O[3]);
-        if (lane == 0) {
-          p[kHeadDim] = M;
-          p[kHeadDim + 1] = L;
-        }
-      }
     }
+  }
+  for (open = __ballot_sync(0xffffffffu, parts > 0); open; open &= open - 1) {
+    const int from = __ffs(open) - 1, w = from >> 1;
+    const int seg = __shfl_sync(0xffffffffu, mine, from), n = __shfl_sync(0xffffffffu, parts, from);
+    const int b = a.by_Hc.div(seg), hc = seg - b * Hc, T = prefix[b + 1] - prefix[b], s0 = prefix[b] * Hc + hc * T;
+    const int kh = a.by_chunks.div(hc), hg = (hc - kh * a.chunks) * kGroup + warp;
+    if (hg >= a.Hg) continue;
+    Joined j;
+    j.add_all(0, 1, n, lane, [&](int i) {
+      const int u = w + i;
+      return part0 + (2 * u + (meta[2 * u] == seg ? 0 : 1)) * kPartFloats + warp * kPitch;
+    });
+    if (s0 >= R0 && s0 + T <= R1)
+      store_head(a, b, kh * a.Hg + hg, kh, j.L, j.O, lane);
+    else
+      j.put(a.parts + ((long)blockIdx.x * 2 + (s0 < R0 ? 0 : 1)) * kPartFloats + warp * kPitch, lane);
+  }
 }
 
-// Joins the (sequence, head) parts that lie in several CTAs: a CTA per (sequence, kv head, group), a warp per head.
-__global__ void __launch_bounds__(kGroup * 32) paged_join_kernel(const AttnArgs a) {
+// Joins the (sequence, head) parts that lie in several CTAs: a CTA per query
+// head, its warps take every fourth part.
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const AttnArgs a) {
+  __shared__ float part[kJoinWarps][kPitch];
   pdl_wait_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, Hc = a.c.Hk * a.chunks;
-  const int b = blockIdx.x / Hc, hc = blockIdx.x % Hc, kh = hc / a.chunks, hg = (hc % a.chunks) * kGroup + warp;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int head = blockIdx.x, b = blockIdx.y, kh = head / a.Hg, hg = head - kh * a.Hg;
+  const int hc = kh * a.chunks + hg / kGroup;
   const int per_cta = a.header[0], p0 = a.header[1 + b], T = a.header[2 + b] - p0;
-  if (T == 0 || hg >= a.Hg) return;
-  const int s0 = p0 * Hc + hc * T, c0 = s0 / per_cta, c1 = (s0 + T - 1) / per_cta;
-  if (c0 == c1) return;
-  float M, L, O[4];
-  join(c1 - c0 + 1, lane, [&](int i) {
-    return a.parts + ((long)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats + warp * kPitch;
-  }, M, L, O);
-  store_head(a, b, kh * a.Hg + hg, kh, L, O, lane);
+  const int s0 = p0 * a.Hc + hc * T, c0 = s0 / per_cta, c1 = (s0 + T - 1) / per_cta;
+  if (T == 0 || c0 == c1) return;
+  Joined j;
+  j.add_all(warp, kJoinWarps, c1 - c0 + 1, lane, [&](int i) {
+    return a.parts + ((long)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats + (hg % kGroup) * kPitch;
+  });
+  j.put(part[warp], lane);
+  __syncthreads();
+  if (warp) return;
+  Joined all;
+  all.add_all(0, 1, kJoinWarps, lane, [&](int i) { return part[i]; });
+  store_head(a, b, head, kh, all.L, all.O, lane);
 }
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -531,14 +571,15 @@ int page_map(CUtensorMap* m, const void* base, const PagedView& c, long stride, 
 
 size_t smem_bytes(int B) {
   return 1024 + (size_t)kWarps * kSlots * 2 * kTileBytes + (size_t)kWarps * 2 * kPartFloats * 4 +
-         kWarps * kSlots * 8 + 3 * kWarps * 4 + (size_t)(B + 1) * 4;
+         kWarps * kSlots * 8 + 3 * kWarps * 4 + (size_t)(2 * B + 1) * 4;
 }
 
-// Sequences whose table holds so few positions that a CTA per (sequence, head)
-// gives a warp two tiles at most are not split: no second kernel.
-bool per_segment(int page, int max_blocks) { return (long)max_blocks * page <= 2L * kWarps * kTile; }
-
-int grid_ctas() { return num_sms(); }
+// A CTA per (sequence, head, group) and no second kernel, when they fit one
+// wave and the table holds so few positions that a warp gets two tiles at most.
+bool per_segment(int segments, int page, int max_blocks) {
+  return segments <= num_sms() && (long)max_blocks * page <= 2L * kWarps * kTile;
+}
+int groups_of(int H, int Hk) { return Hk * ((H / Hk + kGroup - 1) / kGroup); }
 
 size_t header_bytes(int B) { return ((size_t)(B + 2) * 4 + 15) / 16 * 16; }
 
@@ -556,8 +597,9 @@ cudaError_t paged_attn_status(int clear, int* word) {
 using namespace r4q;
 
 extern "C" size_t r4q_paged_flash_decode_workspace_bytes(int B, int H, int Hk, int page, int max_blocks) {
-  if (B < 1 || H < 1 || Hk < 1 || page < 1 || max_blocks < 1 || per_segment(page, max_blocks)) return 0;
-  return header_bytes(B) + (size_t)grid_ctas() * 2 * kPartFloats * 4;
+  if (B < 1 || H < 1 || Hk < 1 || page < 1 || max_blocks < 1) return 0;
+  if (per_segment(B * groups_of(H, Hk), page, max_blocks)) return 0;
+  return header_bytes(B) + (size_t)num_sms() * 2 * kPartFloats * 4;
 }
 
 extern "C" int r4q_paged_flash_decode(const void* q, long ldq, const r4q_paged_cache* cache,
@@ -580,12 +622,15 @@ extern "C" int r4q_paged_flash_decode(const void* q, long ldq, const r4q_paged_c
     return set_error(R4Q_ERR_ALIGN, "paged_flash_decode: q and o must be 16-byte aligned, strides multiples of 8");
   a.Hg = H / a.c.Hk;
   a.chunks = (a.Hg + kGroup - 1) / kGroup;
-  const int Hc = a.c.Hk * a.chunks;
+  const int Hc = a.Hc = groups_of(H, a.c.Hk);
   const long cap = (long)a.c.max_blocks * a.c.page;
   if ((cap / kTile + 1) * B * Hc > 0x7fffffffL - 65536)
     return set_error(R4Q_ERR_ARG, "paged_flash_decode: %d sequences of %ld positions and %d heads are too many tiles",
                      B, cap, Hc);
-  a.per_seg = per_segment(a.c.page, a.c.max_blocks);
+  a.per_seg = per_segment(B * Hc, a.c.page, a.c.max_blocks);
+  a.by_page = fast_div(a.c.page);
+  a.by_Hc = fast_div(Hc);
+  a.by_chunks = fast_div(a.chunks);
   const size_t need = a.per_seg ? 0 : r4q_paged_flash_decode_workspace_bytes(B, H, a.c.Hk, a.c.page, a.c.max_blocks);
   if (need && (!workspace || ws_bytes < need))
     return set_error(R4Q_ERR_CAPACITY, "paged_flash_decode: workspace %zu < %zu bytes", ws_bytes, need);
@@ -621,10 +666,10 @@ extern "C" int r4q_paged_flash_decode(const void* q, long ldq, const r4q_paged_c
     }
   }
   cudaStream_t s = (cudaStream_t)stream;
-  const unsigned ctas = a.per_seg ? (unsigned)(B * Hc) : (unsigned)grid_ctas();
+  const unsigned ctas = a.per_seg ? (unsigned)(B * Hc) : (unsigned)num_sms();
   cudaError_t e = launch_pdl(paged_attn_kernel, dim3(ctas), dim3(kWarps * 32), smem_bytes(B), s, tmk, tmv, a);
   if (e == cudaSuccess && !a.per_seg)
-    e = launch_pdl(paged_join_kernel, dim3((unsigned)(B * Hc)), dim3((unsigned)(min(a.Hg, kGroup) * 32)), 0, s, a);
+    e = launch_pdl(paged_join_kernel, dim3((unsigned)H, (unsigned)B), dim3(kJoinWarps * 32), 0, s, a);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return set_error(R4Q_ERR_CUDA, "paged_attn_kernel: %s", cudaGetErrorString(e));

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent.parent
@@ -63,12 +64,10 @@ class ModelDesc(C.Structure):
         ("tp_size", C.c_int), ("comm", C.c_void_p)]
 
 
-class PagedCache(C.Structure):
-    """r4q_paged_cache (include/r4q.h)."""
-    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("k_stride", C.c_long), ("v_stride", C.c_long),
-                ("n_pages", C.c_int), ("page", C.c_int), ("Hk", C.c_int), ("table", C.c_void_p),
-                ("ld_table", C.c_long), ("seqs", C.c_int), ("max_blocks", C.c_int), ("k_scale", C.c_void_p),
-                ("v_scale", C.c_void_p)]
+# r4q_paged_cache (include/r4q.h) in the platform's C layout: k_pages, v_pages, k_stride, v_stride, n_pages, page, Hk,
+# table, ld_table, seqs, max_blocks, k_scale, v_scale (0: NULL).  The packed bytes are passed as the pointer, which
+# costs a fraction of building a ctypes.Structure per call.
+PAGED_CACHE = struct.Struct("@PPlliiiPliiPP")
 
 _SIGS = {
     "r4q_last_error": (C.c_char_p, []),
@@ -99,9 +98,9 @@ _SIGS = {
     "r4q_dequant_int8": (i32, [vp, vp, vp, i32, i32, vp]),
     "r4q_kv_write_rows": (i32, [vp, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp]),
     "r4q_paged_kv_write": (i32, [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, i64, i64, vp, i64, vp, i64,
-                                 C.POINTER(PagedCache), vp, vp, i32, i32, f32, i32, vp]),
+                                 vp, vp, vp, i32, i32, f32, i32, vp]),
     "r4q_paged_flash_decode_workspace_bytes": (sz_t, [i32, i32, i32, i32, i32]),
-    "r4q_paged_flash_decode": (i32, [vp, i64, C.POINTER(PagedCache), vp, vp, i64, i32, i32, i32, vp, sz_t, vp]),
+    "r4q_paged_flash_decode": (i32, [vp, i64, vp, vp, vp, i64, i32, i32, i32, vp, sz_t, vp]),
     "r4q_paged_status": (i32, [i32]),
     "r4q_kv_copy_pages": (i32, [vp, i64, i64, i64, i64, i32, vp, vp, i32, vp]),
     "r4q_kv_table_set": (i32, [vp, i64, i32, i32, vp, vp, vp, i32, vp]),

@@ -6,7 +6,7 @@ from __future__ import annotations
 import array
 import ctypes as C
 import threading
-from contextlib import nullcontext
+from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
@@ -20,10 +20,13 @@ _ws: dict = {}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def stream_handle(dev: torch.device) -> int:
-    """cudaStream_t of torch's current stream on dev (the raw-handle query
-    costs a fraction of building a torch.cuda.Stream object per call)."""
+def stream_handle(dev) -> int:
+    """cudaStream_t of torch's current stream on dev, a torch.device or an
+    index (the raw-handle query costs a fraction of building a
+    torch.cuda.Stream object per call)."""
     if _raw_stream is not None:
+        if isinstance(dev, int):
+            return _raw_stream(dev)
         return _raw_stream(dev.index if dev.index is not None else torch.cuda.current_device())
     return torch.cuda.current_stream(dev).cuda_stream
 
@@ -411,59 +414,77 @@ def residual_f16(a: torch.Tensor, res: torch.Tensor | None, out: torch.Tensor, s
 
 
 # ------------------------------------------------------------- paged KV cache ---
-def _on(dev: torch.device):
-    """Makes dev the current device for a launch on one of its streams."""
-    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _same_gpu(t: torch.Tensor, *others) -> int:
+    """Index of the one GPU that holds every tensor (None: not given)."""
+    i = t.get_device()
+    for o in others:
+        if o is not None and o.get_device() != i:
+            raise ValueError("all tensors must be on the same CUDA device")
+    if i < 0:
+        raise ValueError("r4q ops take CUDA tensors only (no CPU fallback)")
+    return i
 
 
-def _heads(t: torch.Tensor, name: str, rows: Optional[int] = None, heads: Optional[int] = None,
-           out: bool = False) -> torch.Tensor:
-    """t as fp16 [rows, heads, 128] with its heads side by side and any row
-    stride; an input laid out otherwise is copied, an output refused."""
-    if t.dtype != torch.float16:
+def _run_on(index: int, name: str, *args) -> None:
+    """L.call with the GPU's current stream as the last argument and that GPU current."""
+    if index == torch.cuda.current_device():
+        L.call(name, *args, stream_handle(index))
+    else:
+        with torch.cuda.device(index):
+            L.call(name, *args, stream_handle(index))
+
+
+def _heads(t: torch.Tensor, name: str, rows: Optional[int] = None, heads: Optional[int] = None, out: bool = False):
+    """(t, row stride) of fp16 [rows, heads, 128] with the heads of a row side
+    by side; an input laid out otherwise is copied, an output refused."""
+    if t.dtype is not torch.float16:
         raise TypeError(f"{name} must be float16")
-    if t.dim() != 3 or t.shape[2] != 128 or (rows is not None and t.shape[0] != rows) or \
-            (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be [{rows or 'rows'}, {heads or 'heads'}, 128], got {tuple(t.shape)}")
-    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != 128) or
-                      (t.shape[0] > 1 and t.stride(0) < t.shape[1] * 128)):
+    sh = t.shape
+    if len(sh) != 3 or sh[2] != 128 or (rows is not None and sh[0] != rows) or (heads is not None and sh[1] != heads):
+        raise ValueError(f"{name} must be [{rows or 'rows'}, {heads or 'heads'}, 128], got {tuple(sh)}")
+    width = sh[1] * 128
+    st = t.stride()
+    if st == (width, 128, 1):
+        return t, width
+    if t.numel() and (st[2] != 1 or (sh[1] > 1 and st[1] != 128) or (sh[0] > 1 and st[0] < width)):
         if out:
             raise ValueError(f"{name} must hold the heads of a row side by side")
-        t = t.contiguous()
-    return t
+        return t.contiguous(), width
+    return t, st[0] if sh[0] > 1 else width
 
 
 def _vector(t: torch.Tensor, name: str, dtype: torch.dtype, n: int) -> torch.Tensor:
-    if t.dtype != dtype or tuple(t.shape) != (n,):
+    if t.dtype is not dtype or t.shape != (n,):
         raise ValueError(f"{name} must be {str(dtype)[6:]} [{n}], got {str(t.dtype)[6:]} {tuple(t.shape)}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
-
-
-def _paged_cache(k_pages, v_pages, block_table, k_scale, v_scale) -> L.PagedCache:
-    if k_pages.dtype != torch.uint8 or v_pages.dtype != torch.uint8:
+def _paged_cache(k_pages, v_pages, block_table, k_scale, v_scale):
+    """(packed r4q_paged_cache, Hk, page, max_blocks) of checked tensors."""
+    if k_pages.dtype is not torch.uint8 or v_pages.dtype is not torch.uint8:
         raise TypeError("pages must be uint8 (FP8 E4M3 bytes)")
-    if k_pages.dim() != 4 or k_pages.shape[3] != 128 or v_pages.shape != k_pages.shape:
+    sh = k_pages.shape
+    if len(sh) != 4 or sh[3] != 128 or v_pages.shape != sh:
         raise ValueError("k_pages and v_pages must be [pages, kv heads, page, 128] of one shape, got "
-                         f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
-    P, Hk, page, _ = k_pages.shape
-    for t in (k_pages, v_pages):
-        if t.stride(3) != 1 or t.stride(2) != 128 or (Hk > 1 and t.stride(1) != page * 128):
+                         f"{tuple(sh)} and {tuple(v_pages.shape)}")
+    P, Hk, page, _ = sh
+    ks, vs, inner = k_pages.stride(), v_pages.stride(), (page * 128, 128, 1)
+    for st in (ks, vs):
+        if st[1:] != inner and (st[2:] != inner[1:] or Hk > 1):
             raise ValueError("each page must be contiguous [kv heads, page, 128]")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2:
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2:
         raise TypeError("block_table must be int32 [sequences, blocks]")
     S, nb = block_table.shape
-    if nb and block_table.stride(1) != 1:
+    ld, one = block_table.stride()
+    if one != 1 and nb > 1:
         raise ValueError("block_table rows must be contiguous")
     for s in (k_scale, v_scale):
-        if s is not None and (s.dtype != torch.float32 or tuple(s.shape) != (Hk,) or not s.is_contiguous()):
+        if s is not None and (s.dtype is not torch.float32 or s.shape != (Hk,) or not s.is_contiguous()):
             raise ValueError(f"k_scale and v_scale must be float32 [{Hk}], one per kv head")
-    return L.PagedCache(k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0) if P > 1 else 0,
-                        v_pages.stride(0) if P > 1 else 0, P, page, Hk, block_table.data_ptr(),
-                        block_table.stride(0) if S > 1 else nb, S, nb, _ptr(k_scale), _ptr(v_scale))
+    return L.PAGED_CACHE.pack(k_pages.data_ptr(), v_pages.data_ptr(), ks[0] if P > 1 else 0, vs[0] if P > 1 else 0, P,
+                              page, Hk, block_table.data_ptr(), ld if S > 1 else nb, S, nb,
+                              0 if k_scale is None else k_scale.data_ptr(),
+                              0 if v_scale is None else v_scale.data_ptr()), Hk, page, nb
 
 
 def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -481,49 +502,55 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     tensor, undefined in the rows of padding; q itself for in place) and k in
     ``k_out`` if given.  ``k_scale`` / ``v_scale``: fp32 [Hk], stored byte =
     enc(x / scale), the bytes of the contiguous cache; ``full_range`` keeps
-    256 .. 448 apart, which its codec stores as 448.  Rows, positions and page ids out of range write nothing
-    and are reported by ``check_status``."""
-    ts = [t for t in (k, v, k_pages, v_pages, block_table, positions, rows, q, q_w, k_w, cos, sin, q_out, k_out,
-                      k_scale, v_scale) if t is not None]
-    dev = _require_cuda(*ts)
-    cache = _paged_cache(k_pages, v_pages, block_table, k_scale, v_scale)
-    Hk = cache.Hk
-    k = _heads(k, "k", heads=Hk)
+    256 .. 448 apart, which its codec stores as 448.  Rows, positions and page
+    ids out of range write nothing and are reported by ``check_status``."""
+    gpu = _same_gpu(k, v, k_pages, v_pages, block_table, positions, rows, q, q_w, k_w, cos, sin, q_out, k_out, k_scale,
+                    v_scale)
+    cache, Hk, _, _ = _paged_cache(k_pages, v_pages, block_table, k_scale, v_scale)
+    k, ldk = _heads(k, "k", heads=Hk)
     M = k.shape[0]
-    v = _heads(v, "v", M, Hk)
+    v, ldv = _heads(v, "v", M, Hk)
     positions = _vector(positions, "positions", torch.int64, M)
     if rows is not None:
         rows = _vector(rows, "rows", torch.int32, M)
-    H, flags, tab = 0, L.KV_FULL_RANGE if full_range else 0, (0, 0)
+    H = ldq = ldqo = ldko = tab_stride = tab_rows = 0
+    flags = L.KV_FULL_RANGE if full_range else 0
     if q is not None:
-        q = _heads(q, "q", M)
+        q, ldq = _heads(q, "q", M)
         H = q.shape[1]
-        q_out = torch.empty(M, H, 128, dtype=torch.float16, device=dev) if q_out is None else \
-            _heads(q_out, "q_out", M, H, out=True)
+        if q_out is None:
+            q_out, ldqo = torch.empty(M, H, 128, dtype=torch.float16, device=q.device), H * 128
+        else:
+            q_out, ldqo = _heads(q_out, "q_out", M, H, out=True)
     elif q_out is not None or q_w is not None:
         raise ValueError("q_out and q_w need q")
     if k_out is not None:
-        k_out = _heads(k_out, "k_out", M, Hk, out=True)
+        k_out, ldko = _heads(k_out, "k_out", M, Hk, out=True)
     if k_w is not None or q_w is not None:
         if k_w is None or (q is not None and q_w is None):
             raise ValueError("the norm needs a weight for q and for k")
         for w in (q_w, k_w):
-            if w is not None and (w.dtype != torch.float16 or tuple(w.shape) != (128,) or not w.is_contiguous()):
+            if w is not None and (w.dtype is not torch.float16 or w.shape != (128,) or not w.is_contiguous()):
                 raise ValueError("norm weights must be float16 [128]")
         flags |= L.HEAD_NORM
     if cos is not None or sin is not None:
-        for t in (cos, sin):
-            if t is None or t.dtype != torch.float16 or t.dim() != 2 or t.shape[1] < 64 or t.stride(1) != 1 or \
-                    t.shape != cos.shape or t.stride(0) != cos.stride(0):
-                raise ValueError("cos and sin must be float16 [rows, 64] of one layout")
+        if cos is None or sin is None or cos.dtype is not torch.float16 or sin.dtype is not torch.float16 or \
+                cos.dim() != 2 or cos.shape[1] < 64 or sin.shape != cos.shape or cos.stride(1) != 1 or \
+                sin.stride() != cos.stride():
+            raise ValueError("cos and sin must be float16 [rows, 64] of one layout")
         flags |= L.HEAD_ROPE
-        tab = (cos.stride(0) if cos.shape[0] > 1 else 64, cos.shape[0])
-    with _on(dev):
-        L.call("r4q_paged_kv_write", _ptr(q), 0 if q is None else _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v),
-               _ptr(q_w), _ptr(k_w), _ptr(cos), _ptr(sin), tab[0], tab[1], _ptr(q_out),
-               0 if q_out is None else _ld(q_out), _ptr(k_out), 0 if k_out is None else _ld(k_out), C.byref(cache),
-               _ptr(rows), positions.data_ptr(), M, H, float(eps), flags, stream_handle(dev))
+        tab_rows = cos.shape[0]
+        tab_stride = cos.stride(0) if tab_rows > 1 else 64
+    _run_on(gpu, "r4q_paged_kv_write", _ptr(q), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, _ptr(q_w), _ptr(k_w),
+            _ptr(cos), _ptr(sin), tab_stride, tab_rows, _ptr(q_out), ldqo, _ptr(k_out), ldko, cache, _ptr(rows),
+            positions.data_ptr(), M, H, eps, flags)
     return q_out
+
+
+@lru_cache(maxsize=256)
+def _paged_workspace_bytes(gpu: int, B: int, H: int, Hk: int, page: int, max_blocks: int) -> int:
+    with torch.cuda.device(gpu):
+        return L.LIB.r4q_paged_flash_decode_workspace_bytes(B, H, Hk, page, max_blocks)
 
 
 def paged_flash_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
@@ -537,18 +564,20 @@ def paged_flash_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     table are cut; ``check_status`` reports both.  The workspace comes from
     torch's allocator at every call, so calls on several streams and captured
     graphs share nothing."""
-    dev = _require_cuda(q, k_pages, v_pages, block_table, seq_lens, *(t for t in (k_scale, v_scale, out) if t is not None))
-    q = _heads(q, "q")
+    gpu = _same_gpu(q, k_pages, v_pages, block_table, seq_lens, k_scale, v_scale, out)
+    q, ldq = _heads(q, "q")
     B, H, _ = q.shape
-    cache = _paged_cache(k_pages, v_pages, block_table, k_scale, v_scale)
+    cache, Hk, page, nb = _paged_cache(k_pages, v_pages, block_table, k_scale, v_scale)
     seq_lens = _vector(seq_lens, "seq_lens", torch.int64, B)
-    o = torch.empty(B, H, 128, dtype=torch.float16, device=dev) if out is None else _heads(out, "out", B, H, out=True)
-    with _on(dev):
-        need = L.LIB.r4q_paged_flash_decode_workspace_bytes(B, H, cache.Hk, cache.page, cache.max_blocks)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        L.call("r4q_paged_flash_decode", q.data_ptr(), _ld(q), C.byref(cache), seq_lens.data_ptr(), o.data_ptr(),
-               _ld(o), B, H, L.ATTN_FWHT if fwht else 0, _ptr(ws), need, stream_handle(dev))
-    return o
+    if out is None:
+        out, ldo = torch.empty(B, H, 128, dtype=torch.float16, device=q.device), H * 128
+    else:
+        out, ldo = _heads(out, "out", B, H, out=True)
+    need = _paged_workspace_bytes(gpu, B, H, Hk, page, nb)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _run_on(gpu, "r4q_paged_flash_decode", q.data_ptr(), ldq, cache, seq_lens.data_ptr(), out.data_ptr(), ldo, B, H,
+            L.ATTN_FWHT if fwht else 0, _ptr(ws), need)
+    return out
 
 
 def _host_ints(*lists) -> list:
@@ -574,7 +603,7 @@ def kv_copy_pages(pool: torch.Tensor, src, dst) -> None:
     [..., P, Hk, page, 128], contiguous; src and dst host lists.  A page may be
     copied to several places, but not written twice, nor both read and
     written (r4q_kv_copy_pages)."""
-    dev = _require_cuda(pool)
+    gpu = _same_gpu(pool)
     if pool.dtype != torch.uint8 or pool.dim() < 4 or not pool.is_contiguous():
         raise ValueError("pool must be uint8 [..., pages, kv heads, page, 128] and contiguous")
     s, d = _host_ints(src, dst)
@@ -583,22 +612,19 @@ def kv_copy_pages(pool: torch.Tensor, src, dst) -> None:
     outer = pool.numel() // max(1, P * page_bytes)
     if not pool.numel():
         raise ValueError("empty pool")
-    with _on(dev):
-        L.call("r4q_kv_copy_pages", pool.data_ptr(), outer, P * page_bytes, page_bytes, page_bytes, P,
-               s.buffer_info()[0], d.buffer_info()[0], len(s), stream_handle(dev))
+    _run_on(gpu, "r4q_kv_copy_pages", pool.data_ptr(), outer, P * page_bytes, page_bytes, page_bytes, P,
+            s.buffer_info()[0], d.buffer_info()[0], len(s))
 
 
 def kv_table_set(table: torch.Tensor, rows, cols, values) -> None:
     """table[rows[i], cols[i]] = values[i] in stream order, from host lists
     (r4q_kv_table_set): table int32 [sequences, blocks] on the device; no cell twice."""
-    dev = _require_cuda(table)
+    gpu = _same_gpu(table)
     if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
         raise ValueError("table must be int32 [sequences, blocks] with contiguous rows")
     r, c, v = _host_ints(rows, cols, values)
-    with _on(dev):
-        L.call("r4q_kv_table_set", table.data_ptr(), table.stride(0) if table.shape[0] > 1 else table.shape[1],
-               table.shape[0], table.shape[1], r.buffer_info()[0], c.buffer_info()[0], v.buffer_info()[0], len(r),
-               stream_handle(dev))
+    _run_on(gpu, "r4q_kv_table_set", table.data_ptr(), table.stride(0) if table.shape[0] > 1 else table.shape[1],
+            table.shape[0], table.shape[1], r.buffer_info()[0], c.buffer_info()[0], v.buffer_info()[0], len(r))
 
 
 # ----------------------------------------------------------- token likelihoods ---
@@ -628,21 +654,20 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
         raise TypeError(f"logits must be float16, bfloat16 or float32, not {logits.dtype}")
     if logits.dim() != 2:
         raise ValueError("logits must be [rows, vocabulary]")
-    dev = _require_cuda(logits) if tokens is None else _require_cuda(logits, tokens)
+    gpu = _same_gpu(logits, tokens)
     M, V = logits.shape
     if V < 1 or not 0 <= k <= min(V, L.MAX_TOP):
         raise ValueError(f"k must be in [0, {min(V, L.MAX_TOP)}], got {k} (vocabulary {V})")
-    if (V > 1 and logits.stride(1) != 1) or (M > 1 and logits.stride(0) < V):
-        logits = logits.contiguous()
+    ld, one = logits.stride()
+    if (one != 1 and V > 1) or (ld < V and M > 1):
+        logits, ld = logits.contiguous(), V
+    dev, logprob, rank = logits.device, None, None
+    entropy = torch.empty(M, dtype=torch.float32, device=dev)
     if tokens is not None:
         tokens = _vector(tokens, "tokens", torch.int64, M)
-    f32 = dict(dtype=torch.float32, device=dev)
-    i64 = dict(dtype=torch.int64, device=dev)
-    r = TokenLogprobs(None if tokens is None else torch.empty(M, **f32),
-                      None if tokens is None else torch.empty(M, **i64), torch.empty(M, **f32),
-                      torch.empty(M, k, **i64), torch.empty(M, k, **f32))
-    with _on(dev):
-        L.call("r4q_token_logprobs", logits.data_ptr(), ty, logits.stride(0) if M > 1 else V, _ptr(tokens), M, V, k,
-               _ptr(r.logprob), _ptr(r.rank), r.entropy.data_ptr(), r.top_ids.data_ptr(), r.top_logprobs.data_ptr(),
-               stream_handle(dev))
-    return r
+        logprob, rank = torch.empty_like(entropy), torch.empty_like(tokens)
+    top_ids = torch.empty(M, k, dtype=torch.int64, device=dev)
+    top = torch.empty(M, k, dtype=torch.float32, device=dev)
+    _run_on(gpu, "r4q_token_logprobs", logits.data_ptr(), ty, ld if M > 1 else V, _ptr(tokens), M, V, k, _ptr(logprob),
+            _ptr(rank), entropy.data_ptr(), top_ids.data_ptr(), top.data_ptr())
+    return TokenLogprobs(logprob, rank, entropy, top_ids, top)

@@ -123,9 +123,9 @@ P16 = C.c_void_p(256)                             # never dereferenced: validati
 
 def cache(**kw):
     d = dict(k_pages=256, v_pages=256, k_stride=0, v_stride=0, n_pages=4, page=16, Hk=2, table=256, ld_table=4, seqs=3,
-             max_blocks=4, k_scale=None, v_scale=None)
-    d.update(kw)
-    return C.byref(L.PagedCache(**d))
+             max_blocks=4, k_scale=0, v_scale=0)
+    d.update({k: v or 0 for k, v in kw.items()})
+    return L.PAGED_CACHE.pack(*d.values())
 
 
 def attn(c=None, q=P16, ldq=512, seq=P16, o=P16, ldo=512, B=2, H=4, flags=0, ws=P16, ws_bytes=1 << 40):
