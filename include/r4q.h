@@ -258,7 +258,7 @@ enum { R4Q_KV_FULL_RANGE = 8 };
  * stores every |x / scale| from 248 on as 448; with R4Q_KV_FULL_RANGE 256 .. 448
  * are stored as E4M3 has them (all readers decode both), for scales that bring
  * the largest values near 448.
- * A token with pos[m] < 0 is padding: nothing of it is read or written.  A row,
+ * A token with pos[m] < 0 is padding: nothing of it is written.  A row,
  * position, page or table row out of range writes nothing and is reported by
  * r4q_paged_status.  Two tokens of one call must not name one position.
  * 16-byte aligned pointers, row strides in multiples of 8 elements. */

@@ -34,6 +34,7 @@ struct WriteArgs {
   const int* rows;
   const long long* pos;
   int M, H, groups;                // groups of kHeads heads per token
+  FastDiv by_groups, by_page;
   float eps;
   int flags;
 };
@@ -60,58 +61,66 @@ __device__ __forceinline__ float head_rrms(const float (&x)[4], float eps, int l
   }
   return rsqrtf((s[0] + s[1]) / (float)kHeadDim + eps);
 }
-// The cache codec (fp8_encode), or with `full` the same rounding without its
-// saturation of the whole top binade: 256 .. 448 are kept as E4M3 has them.
-__device__ __forceinline__ uint32_t encode(float x, bool full) {
-  const uint32_t r = fp8_encode(x);
-  if (!full || (r & 0x7Fu) != 0x7Eu) return r;
-  const uint32_t f = __float_as_uint(fminf(fabsf(x), 448.0f));      // 248 .. 448, NaN as 448
-  const uint32_t m = (f >> 20) + ((f >> 19) & 1u);                  // exponent and 3 bits, ties away from zero
-  return (r & 0x80u) | (m - (120u << 3));
+// The value that the cache codec (fp8_encode) stores for x: three mantissa bits,
+// ties away from zero, a signed zero below 2^-6, and 448 from 256 on, or with
+// `full` for what exceeds it only.  The hardware conversion of such a value is
+// exact, so rounding on the float and converting in pairs gives fp8_encode's
+// bytes in half its instructions.
+__device__ __forceinline__ float stored(float x, bool full) {
+  const uint32_t u = __float_as_uint(fmaxf(-448.0f, fminf(448.0f, x)));
+  const float r = __uint_as_float((u + 0x80000u) & 0xfff00000u);
+  const float top = !full && fabsf(r) >= 256.0f ? 448.0f : fabsf(r);
+  return copysignf(fabsf(r) < 0x1p-6f ? 0.0f : top, r);
 }
 __device__ __forceinline__ uint32_t encode2(float a, float b, const float* scale, int kh, bool full) {
-  const float s = scale ? scale[kh] : 1.0f;
-  return encode(scale ? a / s : a, full) | (encode(scale ? b / s : b, full) << 8);
+  if (scale) {
+    const float s = scale[kh];
+    a = a / s;
+    b = b / s;
+  }
+  uint16_t d;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(stored(b, full)), "f"(stored(a, full)));
+  return d;
 }
 
 __global__ void __launch_bounds__(256) paged_write_kernel(const WriteArgs a) {
-  const int lane = threadIdx.x & 31;
-  const long w = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const long m = w / a.groups;
+  const int lane = threadIdx.x & 31, w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int m = a.by_groups.div(w), nh = a.H + 2 * a.c.Hk;
   if (m >= a.M) return;
-  const int h0 = (int)(w - m * a.groups) * kHeads, nh = a.H + 2 * a.c.Hk;
+  pdl_wait_trigger();
+  const int h0 = (w - m * a.groups) * kHeads;
   const long long pos = a.pos[m];
+  const int row = a.rows ? a.rows[m] : m;
+  uint32_t x32[kHeads][2];                           // before the position's lookups: independent of them
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const int h = h0 + i;
+    const __half* src = h < a.H            ? a.q + m * a.ldq + (long)h * kHeadDim
+                        : h < a.H + a.c.Hk ? a.k + m * a.ldk + (long)(h - a.H) * kHeadDim
+                                           : a.v + m * a.ldv + (long)(h - a.H - a.c.Hk) * kHeadDim;
+    const uint32_t* s32 = reinterpret_cast<const uint32_t*>(src);
+    x32[i][0] = h < nh ? s32[lane] : 0u;
+    x32[i][1] = h < nh ? s32[lane + 32] : 0u;
+  }
   if (pos < 0) return;
-  const long row = a.rows ? a.rows[m] : m;
   bool ok = row >= 0 && row < a.c.seqs && pos < (long long)a.c.max_blocks * a.c.page;
   if (ok && (a.flags & R4Q_HEAD_ROPE)) ok = pos < a.tab_rows;
-  int pg = 0;
+  int pg = 0, in_page = 0;
+  float2 c{1.f, 1.f}, s{0.f, 0.f};
   if (ok) {
-    pg = a.c.table[row * a.c.ld_table + (int)pos / a.c.page];
+    const int blk = a.by_page.div((int)pos);
+    in_page = (int)pos - blk * a.c.page;
+    pg = a.c.table[row * a.c.ld_table + blk];
+    if (a.flags & R4Q_HEAD_ROPE) {
+      c = __half22float2(u32_as_h2(reinterpret_cast<const uint32_t*>(a.cos_tab + pos * a.tab_stride)[lane]));
+      s = __half22float2(u32_as_h2(reinterpret_cast<const uint32_t*>(a.sin_tab + pos * a.tab_stride)[lane]));
+    }
     ok = pg >= 0 && pg < a.c.n_pages;
   }
   if (!ok) {
     if (lane == 0) atomicOr(&g_write_status, kPagedBadPage);
     return;
   }
-  float x[kHeads][4];
-#pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
-    const int h = h0 + i;
-    if (h >= nh) break;
-    const __half* src = h < a.H               ? a.q + m * a.ldq + (long)h * kHeadDim
-                        : h < a.H + a.c.Hk    ? a.k + m * a.ldk + (long)(h - a.H) * kHeadDim
-                                              : a.v + m * a.ldv + (long)(h - a.H - a.c.Hk) * kHeadDim;
-    const uint32_t* s32 = reinterpret_cast<const uint32_t*>(src);
-    const float2 lo = __half22float2(u32_as_h2(s32[lane])), hi = __half22float2(u32_as_h2(s32[lane + 32]));
-    x[i][0] = lo.x; x[i][1] = lo.y; x[i][2] = hi.x; x[i][3] = hi.y;
-  }
-  float2 c{1.f, 1.f}, s{0.f, 0.f};
-  if (a.flags & R4Q_HEAD_ROPE) {
-    c = __half22float2(u32_as_h2(reinterpret_cast<const uint32_t*>(a.cos_tab + pos * a.tab_stride)[lane]));
-    s = __half22float2(u32_as_h2(reinterpret_cast<const uint32_t*>(a.sin_tab + pos * a.tab_stride)[lane]));
-  }
-  const long in_page = (long)((int)pos % a.c.page) * kHeadDim;
   const bool full = a.flags & R4Q_KV_FULL_RANGE;
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
@@ -119,7 +128,8 @@ __global__ void __launch_bounds__(256) paged_write_kernel(const WriteArgs a) {
     if (h >= nh) break;
     const bool is_q = h < a.H, is_v = h >= a.H + a.c.Hk;
     const int kh = is_q ? 0 : is_v ? h - a.H - a.c.Hk : h - a.H;
-    float(&v)[4] = x[i];
+    const float2 x0 = __half22float2(u32_as_h2(x32[i][0])), x1 = __half22float2(u32_as_h2(x32[i][1]));
+    float v[4] = {x0.x, x0.y, x1.x, x1.y};
     if (!is_v) {
       if (a.flags & R4Q_HEAD_NORM) {
         const float rrms = head_rrms(v, a.eps, lane);
@@ -146,28 +156,44 @@ __global__ void __launch_bounds__(256) paged_write_kernel(const WriteArgs a) {
       o32[lane + 32] = h2_as_u32(__floats2half2_rn(v[2], v[3]));
     }
     if (is_q) continue;
-    uint8_t* dst = (is_v ? a.c.v + pg * a.c.v_stride : a.c.k + pg * a.c.k_stride) +
-                   (long)kh * a.c.page * kHeadDim + in_page;
+    // codes of elements 2l, 2l+1 and 64+2l, 65+2l: even lanes store four of the
+    // first half with their neighbour's, odd lanes of the second
     const float* scale = is_v ? a.c.v_scale : a.c.k_scale;
-    reinterpret_cast<uint16_t*>(dst)[lane] = (uint16_t)encode2(v[0], v[1], scale, kh, full);
-    reinterpret_cast<uint16_t*>(dst)[lane + 32] = (uint16_t)encode2(v[2], v[3], scale, kh, full);
+    const uint32_t lo = encode2(v[0], v[1], scale, kh, full), hi = encode2(v[2], v[3], scale, kh, full);
+    const bool even = !(lane & 1);
+    const uint32_t got = __shfl_xor_sync(0xffffffffu, even ? hi : lo, 1);
+    uint8_t* dst = (is_v ? a.c.v + pg * a.c.v_stride : a.c.k + pg * a.c.k_stride) +
+                   ((long)kh * a.c.page + in_page) * kHeadDim;
+    reinterpret_cast<uint32_t*>(dst)[even ? lane >> 1 : 16 + (lane >> 1)] = even ? lo | got << 16 : got | hi << 16;
   }
 }
 
 // ------------------------------------------------------------- page copies
+// Bound: HBM, every byte read and written once.  A CTA copies 16 KB of a page,
+// four 16-byte loads a thread in flight: a fork's few pages over all layers
+// (tens of MB) then still fill the SMs.  The moves travel in the launch's
+// parameters: no copy to the device, and nothing to keep alive behind the call.
 constexpr int kMaxMoves = 448;          // (src, dst) pairs in one launch's parameters (3.5 KB)
+constexpr int kCopyVecs = 4, kCopyChunk = 256 * kCopyVecs;   // 16-byte words of a CTA
 struct Moves {
   int src[kMaxMoves], dst[kMaxMoves];
 };
 
 __global__ void __launch_bounds__(256)
-    copy_pages_kernel(uint8_t* pool, long outer_stride, long page_stride, long page_bytes,
+    copy_pages_kernel(uint8_t* pool, long outer_stride, long page_stride, long words,
                       const __grid_constant__ Moves mv) {
-  const int i = blockIdx.x;
-  uint8_t* base = pool + (long)blockIdx.y * outer_stride;
-  const uint4* s = reinterpret_cast<const uint4*>(base + (long)mv.src[i] * page_stride);
-  uint4* d = reinterpret_cast<uint4*>(base + (long)mv.dst[i] * page_stride);
-  for (long j = threadIdx.x; j < page_bytes / 16; j += blockDim.x) d[j] = s[j];
+  pdl_wait_trigger();
+  uint8_t* base = pool + (long)blockIdx.z * outer_stride;
+  const uint4* s = reinterpret_cast<const uint4*>(base + (long)mv.src[blockIdx.y] * page_stride);
+  uint4* d = reinterpret_cast<uint4*>(base + (long)mv.dst[blockIdx.y] * page_stride);
+  const long at = (long)blockIdx.x * kCopyChunk + threadIdx.x;
+  uint4 v[kCopyVecs];
+#pragma unroll
+  for (int j = 0; j < kCopyVecs; ++j)
+    if (at + 256 * j < words) v[j] = s[at + 256 * j];
+#pragma unroll
+  for (int j = 0; j < kCopyVecs; ++j)
+    if (at + 256 * j < words) d[at + 256 * j] = v[j];
 }
 
 constexpr int kMaxCells = 320;
@@ -175,6 +201,7 @@ struct Cells {
   int r[kMaxCells], c[kMaxCells], v[kMaxCells];
 };
 __global__ void table_set_kernel(int* table, long ld, int n, const __grid_constant__ Cells cells) {
+  pdl_wait_trigger();
   for (int i = threadIdx.x; i < n; i += blockDim.x) table[cells.r[i] * ld + cells.c[i]] = cells.v[i];
 }
 
@@ -242,10 +269,17 @@ extern "C" int r4q_paged_kv_write(const void* q, long ldq, const void* k, long l
   a.rows = rows; a.pos = pos;
   a.M = M; a.H = has_q ? H : 0; a.eps = eps; a.flags = flags;
   a.groups = (a.H + 2 * a.c.Hk + kHeads - 1) / kHeads;
+  a.by_groups = fast_div(a.groups);
+  a.by_page = fast_div(a.c.page);
   const long warps = (long)M * a.groups;
-  if ((warps + 7) / 8 > 0x7fffffffL) return set_error(R4Q_ERR_ARG, "paged_kv_write: M * heads too large");
-  paged_write_kernel<<<(unsigned)((warps + 7) / 8), 256, 0, (cudaStream_t)stream>>>(a);
-  return check_launch("paged_write_kernel");
+  if (warps > 0x7ffffff0L) return set_error(R4Q_ERR_ARG, "paged_kv_write: %d tokens of %d heads are too many", M, H);
+  const cudaError_t e =
+      launch_pdl(paged_write_kernel, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, (cudaStream_t)stream, a);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(R4Q_ERR_CUDA, "paged_write_kernel: %s", cudaGetErrorString(e));
+  }
+  return R4Q_OK;
 }
 
 extern "C" int r4q_kv_copy_pages(void* pool, long outer, long outer_stride, long page_stride, long page_bytes,
@@ -256,7 +290,9 @@ extern "C" int r4q_kv_copy_pages(void* pool, long outer, long outer_stride, long
     return set_error(R4Q_ERR_ARG, "kv_copy_pages: strides below a page's %ld bytes", page_bytes);
   if (!aligned(pool, 16) || page_bytes % 16 || page_stride % 16 || outer_stride % 16)
     return set_error(R4Q_ERR_ALIGN, "kv_copy_pages: pool, page size and strides must be multiples of 16 bytes");
-  if (outer > 65535) return set_error(R4Q_ERR_ARG, "kv_copy_pages: %ld pools (at most 65535)", outer);
+  const long chunks = (page_bytes / 16 + kCopyChunk - 1) / kCopyChunk;
+  if (outer > 65535 || chunks > 0x7fffffffL)
+    return set_error(R4Q_ERR_ARG, "kv_copy_pages: %ld pools (at most 65535) of %ld-byte pages", outer, page_bytes);
   std::vector<uint8_t> seen(n ? n_pages : 0, 0);     // 1: read, 2: written
   for (int i = 0; i < n; ++i) {
     if (src[i] < 0 || src[i] >= n_pages || dst[i] < 0 || dst[i] >= n_pages)
@@ -274,10 +310,13 @@ extern "C" int r4q_kv_copy_pages(void* pool, long outer, long outer_stride, long
     Moves mv;
     memcpy(mv.src, src + at, part * sizeof(int));
     memcpy(mv.dst, dst + at, part * sizeof(int));
-    copy_pages_kernel<<<dim3(part, (unsigned)outer), 256, 0, (cudaStream_t)stream>>>(
-        (uint8_t*)pool, outer_stride, page_stride, page_bytes, mv);
-    const int st = check_launch("copy_pages_kernel");
-    if (st) return st;
+    const cudaError_t e =
+        launch_pdl(copy_pages_kernel, dim3((unsigned)chunks, part, (unsigned)outer), dim3(256), 0,
+                   (cudaStream_t)stream, (uint8_t*)pool, outer_stride, page_stride, page_bytes / 16, mv);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return set_error(R4Q_ERR_CUDA, "copy_pages_kernel: %s", cudaGetErrorString(e));
+    }
   }
   return R4Q_OK;
 }
@@ -296,9 +335,11 @@ extern "C" int r4q_kv_table_set(int* table, long ld, int rows, int cols, const i
     memcpy(cells.r, r + at, part * sizeof(int));
     memcpy(cells.c, c + at, part * sizeof(int));
     memcpy(cells.v, v + at, part * sizeof(int));
-    table_set_kernel<<<1, 256, 0, (cudaStream_t)stream>>>(table, ld, part, cells);
-    const int st = check_launch("table_set_kernel");
-    if (st) return st;
+    const cudaError_t e = launch_pdl(table_set_kernel, dim3(1), dim3(256), 0, (cudaStream_t)stream, table, ld, part, cells);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return set_error(R4Q_ERR_CUDA, "table_set_kernel: %s", cudaGetErrorString(e));
+    }
   }
   return R4Q_OK;
 }

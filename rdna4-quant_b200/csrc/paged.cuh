@@ -12,6 +12,19 @@ constexpr int kHeadDim = 128;
 constexpr int kPagedTimeout = 1;   // a bounded wait gave up
 constexpr int kPagedBadPage = 2;   // a row, position, length or page id outside the cache
 
+// x / d for 0 <= x < 2^31 by a multiplication: m = ceil(2^(31 + s) / d), 2^(s-1) < d <= 2^s
+// (Granlund and Montgomery, Division by invariant integers using multiplication, 1994)
+struct FastDiv {
+  uint32_t m;
+  int s;
+  __device__ __forceinline__ int div(int x) const { return (int)(((uint64_t)m * (uint32_t)x) >> (31 + s)); }
+};
+inline FastDiv fast_div(uint32_t d) {
+  int s = 0;
+  while ((1ull << s) < d) ++s;
+  return FastDiv{(uint32_t)(((1ull << (31 + s)) + d - 1) / d), s};
+}
+
 struct PagedView {
   uint8_t *k, *v;
   long k_stride, v_stride;         // bytes between pages

@@ -55,19 +55,6 @@ constexpr int kMaxBatch = 2048;
 constexpr int kJoinWarps = 4;
 constexpr int kWaitPolls = 1 << 22;
 
-// x / d for 0 <= x < 2^31 by a multiplication: m = ceil(2^(31 + s) / d), 2^(s-1) < d <= 2^s
-// (Granlund and Montgomery, Division by invariant integers using multiplication, 1994)
-struct FastDiv {
-  uint32_t m;
-  int s;
-  __device__ __forceinline__ int div(int x) const { return (int)(((uint64_t)m * (uint32_t)x) >> (31 + s)); }
-};
-FastDiv fast_div(uint32_t d) {
-  int s = 0;
-  while ((1ull << s) < d) ++s;
-  return FastDiv{(uint32_t)(((1ull << (31 + s)) + d - 1) / d), s};
-}
-
 struct AttnArgs {
   const __half* q;
   long ldq;
