@@ -13,16 +13,17 @@ namespace {
 __device__ int g_write_status;
 
 // ---------------------------------------------------------------- KV write
-// A warp takes kHeads consecutive heads of one token (H of q, Hk of k, Hk of v),
-// so that the token's position, page and rotation row are looked up once and
-// kHeads loads are in flight together.  Lane l holds elements 2l, 2l + 1 and
-// 64 + 2l, 65 + 2l: 4-byte accesses that a warp makes contiguous, and the RoPE
-// partners i, i + 64 in one lane.  Norm and rotation are those of head_kernel
-// (r4q_head_norm_rope) to the bit, so a paged cache holds the bytes that the
-// contiguous one would: the sum of squares runs over elements r, r + 32,
-// r + 64, r + 96 first and then pairwise over r, which here takes the values
-// of lane l ^ 16 and a butterfly over two partial sums per lane.
-constexpr int kHeads = 4;
+// A warp takes two pairs of heads of one token (H of q, Hk of k, Hk of v), a
+// half-warp per head, so that the token's position, page and rotation row are
+// looked up once and eight loads a lane are in flight together.  Lane s of a half holds
+// elements 2s, 2s + 1 of each 32-block: the RoPE partners i, i + 64 and the terms
+// that head_kernel (r4q_head_norm_rope) adds in one lane are in one lane here too,
+// and a butterfly over the half finishes the sum of squares in its order.  Norm
+// and rotation equal that kernel's to the bit, so a paged cache holds the bytes
+// that the contiguous one would.  Bound: issue slots (a warp per head with the
+// loads a lane-strided 2 bytes took 184 instructions a head).
+constexpr int kPairs = 2;
+constexpr int kHeads = 2 * kPairs;
 struct WriteArgs {
   const __half *q, *k, *v;
   long ldq, ldk, ldv;
@@ -39,28 +40,6 @@ struct WriteArgs {
   int flags;
 };
 
-// rsqrt(mean(x^2) + eps) of the head that the warp holds as (2l, 2l+1, 64+2l, 65+2l)
-__device__ __forceinline__ float head_rrms(const float (&x)[4], float eps, int lane) {
-  float s[2];
-#pragma unroll
-  for (int a = 0; a < 2; ++a) {
-    const float y0 = __shfl_xor_sync(0xffffffffu, x[a], 16), y1 = __shfl_xor_sync(0xffffffffu, x[2 + a], 16);
-    const bool low = lane < 16;
-    const float v0 = low ? x[a] : y0, v1 = low ? y0 : x[a], v2 = low ? x[2 + a] : y1, v3 = low ? y1 : x[2 + a];
-    float ss = 0.0f;
-    ss += v0 * v0;
-    ss += v1 * v1;
-    ss += v2 * v2;
-    ss += v3 * v3;
-    s[a] = ss;
-  }
-#pragma unroll
-  for (int d = 8; d > 0; d >>= 1) {
-    s[0] += __shfl_xor_sync(0xffffffffu, s[0], d);
-    s[1] += __shfl_xor_sync(0xffffffffu, s[1], d);
-  }
-  return rsqrtf((s[0] + s[1]) / (float)kHeadDim + eps);
-}
 // The value that the cache codec (fp8_encode) stores for x: three mantissa bits,
 // ties away from zero, a signed zero below 2^-6, and 448 from 256 on, or with
 // `full` for what exceeds it only.  The hardware conversion of such a value is
@@ -83,88 +62,120 @@ __device__ __forceinline__ uint32_t encode2(float a, float b, const float* scale
   return d;
 }
 
+__device__ __forceinline__ float2 half2_of(uint32_t u) { return __half22float2(u32_as_h2(u)); }
+
 __global__ void __launch_bounds__(256) paged_write_kernel(const WriteArgs a) {
-  const int lane = threadIdx.x & 31, w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, sl = lane & 15, half = lane >> 4;
+  const int w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const int m = a.by_groups.div(w), nh = a.H + 2 * a.c.Hk;
   if (m >= a.M) return;
   pdl_wait_trigger();
   const int h0 = (w - m * a.groups) * kHeads;
   const long long pos = a.pos[m];
   const int row = a.rows ? a.rows[m] : m;
-  uint32_t x32[kHeads][2];                           // before the position's lookups: independent of them
+  uint32_t x32[kPairs][4];                           // before the position's lookups: independent of them
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
-    const int h = h0 + i;
+  for (int i = 0; i < kPairs; ++i) {
+    const int h = h0 + 2 * i + half;
     const __half* src = h < a.H            ? a.q + m * a.ldq + (long)h * kHeadDim
                         : h < a.H + a.c.Hk ? a.k + m * a.ldk + (long)(h - a.H) * kHeadDim
                                            : a.v + m * a.ldv + (long)(h - a.H - a.c.Hk) * kHeadDim;
-    const uint32_t* s32 = reinterpret_cast<const uint32_t*>(src);
-    x32[i][0] = h < nh ? s32[lane] : 0u;
-    x32[i][1] = h < nh ? s32[lane + 32] : 0u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x32[i][j] = h < nh ? reinterpret_cast<const uint32_t*>(src)[sl + 16 * j] : 0u;
   }
   if (pos < 0) return;
+  const bool norm = a.flags & R4Q_HEAD_NORM, rope = a.flags & R4Q_HEAD_ROPE, full = a.flags & R4Q_KV_FULL_RANGE;
   bool ok = row >= 0 && row < a.c.seqs && pos < (long long)a.c.max_blocks * a.c.page;
-  if (ok && (a.flags & R4Q_HEAD_ROPE)) ok = pos < a.tab_rows;
+  if (ok && rope) ok = pos < a.tab_rows;
   int pg = 0, in_page = 0;
-  float2 c{1.f, 1.f}, s{0.f, 0.f};
+  float2 c[2] = {{1.f, 1.f}, {1.f, 1.f}}, s[2] = {{0.f, 0.f}, {0.f, 0.f}};
   if (ok) {
     const int blk = a.by_page.div((int)pos);
     in_page = (int)pos - blk * a.c.page;
     pg = a.c.table[row * a.c.ld_table + blk];
-    if (a.flags & R4Q_HEAD_ROPE) {
-      c = __half22float2(u32_as_h2(reinterpret_cast<const uint32_t*>(a.cos_tab + pos * a.tab_stride)[lane]));
-      s = __half22float2(u32_as_h2(reinterpret_cast<const uint32_t*>(a.sin_tab + pos * a.tab_stride)[lane]));
-    }
+    if (rope)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        c[j] = half2_of(reinterpret_cast<const uint32_t*>(a.cos_tab + pos * a.tab_stride)[sl + 16 * j]);
+        s[j] = half2_of(reinterpret_cast<const uint32_t*>(a.sin_tab + pos * a.tab_stride)[sl + 16 * j]);
+      }
     ok = pg >= 0 && pg < a.c.n_pages;
   }
   if (!ok) {
     if (lane == 0) atomicOr(&g_write_status, kPagedBadPage);
     return;
   }
-  const bool full = a.flags & R4Q_KV_FULL_RANGE;
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
-    const int h = h0 + i;
-    if (h >= nh) break;
-    const bool is_q = h < a.H, is_v = h >= a.H + a.c.Hk;
+  for (int i = 0; i < kPairs; ++i) {
+    const int h = h0 + 2 * i + half;
+    if (h0 + 2 * i >= nh) break;                     // uniform; from here on the halves stay together
+    const bool in = h < nh, is_q = h < a.H, is_v = h >= a.H + a.c.Hk;
     const int kh = is_q ? 0 : is_v ? h - a.H - a.c.Hk : h - a.H;
-    const float2 x0 = __half22float2(u32_as_h2(x32[i][0])), x1 = __half22float2(u32_as_h2(x32[i][1]));
-    float v[4] = {x0.x, x0.y, x1.x, x1.y};
-    if (!is_v) {
-      if (a.flags & R4Q_HEAD_NORM) {
-        const float rrms = head_rrms(v, a.eps, lane);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = half2_of(x32[i][j]);
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+    }
+    if (h0 + 2 * i < a.H + a.c.Hk) {                 // a q or k head among the two
+      if (norm) {
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s0 += v[2 * j] * v[2 * j];
+          s1 += v[2 * j + 1] * v[2 * j + 1];
+        }
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) {
+          s0 += __shfl_xor_sync(0xffffffffu, s0, d);
+          s1 += __shfl_xor_sync(0xffffffffu, s1, d);
+        }
+        const float rrms = rsqrtf((s0 + s1) / (float)kHeadDim + a.eps);
         const uint32_t* w32 = reinterpret_cast<const uint32_t*>(is_q ? a.qw : a.kw);
-        const float2 lo = __half22float2(u32_as_h2(w32[lane])), hi = __half22float2(u32_as_h2(w32[lane + 32]));
-        v[0] = v[0] * rrms * lo.x;
-        v[1] = v[1] * rrms * lo.y;
-        v[2] = v[2] * rrms * hi.x;
-        v[3] = v[3] * rrms * hi.y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = half2_of(w32[sl + 16 * j]);
+          v[2 * j] = is_v ? v[2 * j] : v[2 * j] * rrms * f.x;
+          v[2 * j + 1] = is_v ? v[2 * j + 1] : v[2 * j + 1] * rrms * f.y;
+        }
       }
-      if (a.flags & R4Q_HEAD_ROPE) {
-        const float e0 = v[0], o0 = v[2], e1 = v[1], o1 = v[3];
-        v[0] = e0 * c.x - o0 * s.x;
-        v[2] = o0 * c.x + e0 * s.x;
-        v[1] = e1 * c.y - o1 * s.y;
-        v[3] = o1 * c.y + e1 * s.y;
+      if (rope && !is_v) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float e0 = v[2 * j], o0 = v[2 * j + 4], e1 = v[2 * j + 1], o1 = v[2 * j + 5];
+          v[2 * j] = e0 * c[j].x - o0 * s[j].x;
+          v[2 * j + 4] = o0 * c[j].x + e0 * s[j].x;
+          v[2 * j + 1] = e1 * c[j].y - o1 * s[j].y;
+          v[2 * j + 5] = o1 * c[j].y + e1 * s[j].y;
+        }
       }
+      __half* out = is_q ? a.q_out + m * a.ldqo + (long)h * kHeadDim
+                         : !is_v && a.k_out ? a.k_out + m * a.ldko + (long)kh * kHeadDim : nullptr;
+      if (in && out)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          reinterpret_cast<uint32_t*>(out)[sl + 16 * j] = h2_as_u32(__floats2half2_rn(v[2 * j], v[2 * j + 1]));
     }
-    __half* out = is_q ? a.q_out + m * a.ldqo + (long)h * kHeadDim
-                       : !is_v && a.k_out ? a.k_out + m * a.ldko + (long)kh * kHeadDim : nullptr;
-    if (out) {
-      uint32_t* o32 = reinterpret_cast<uint32_t*>(out);
-      o32[lane] = h2_as_u32(__floats2half2_rn(v[0], v[1]));
-      o32[lane + 32] = h2_as_u32(__floats2half2_rn(v[2], v[3]));
-    }
-    if (is_q) continue;
-    // codes of elements 2l, 2l+1 and 64+2l, 65+2l: even lanes store four of the
-    // first half with their neighbour's, odd lanes of the second
+    if (h0 + 2 * i + 1 < a.H) continue;              // two q heads
+    // a lane has the codes of elements 2s, 2s + 1 of four 32-blocks: even lanes
+    // store four bytes of blocks 0 and 1 with their neighbour's, odd lanes of 2 and 3
     const float* scale = is_v ? a.c.v_scale : a.c.k_scale;
-    const uint32_t lo = encode2(v[0], v[1], scale, kh, full), hi = encode2(v[2], v[3], scale, kh, full);
+    uint32_t e01 = 0, e23 = 0;
+    if (in && !is_q) {
+      e01 = encode2(v[0], v[1], scale, kh, full) | encode2(v[2], v[3], scale, kh, full) << 16;
+      e23 = encode2(v[4], v[5], scale, kh, full) | encode2(v[6], v[7], scale, kh, full) << 16;
+    }
     const bool even = !(lane & 1);
-    const uint32_t got = __shfl_xor_sync(0xffffffffu, even ? hi : lo, 1);
-    uint8_t* dst = (is_v ? a.c.v + pg * a.c.v_stride : a.c.k + pg * a.c.k_stride) +
-                   ((long)kh * a.c.page + in_page) * kHeadDim;
-    reinterpret_cast<uint32_t*>(dst)[even ? lane >> 1 : 16 + (lane >> 1)] = even ? lo | got << 16 : got | hi << 16;
+    const uint32_t own = even ? e01 : e23, got = __shfl_xor_sync(0xffffffffu, even ? e23 : e01, 1);
+    if (in && !is_q) {
+      uint8_t* dst = (is_v ? a.c.v + pg * a.c.v_stride : a.c.k + pg * a.c.k_stride) +
+                     ((long)kh * a.c.page + in_page) * kHeadDim;
+      uint32_t* d32 = reinterpret_cast<uint32_t*>(dst) + (even ? 0 : 16) + (sl >> 1);
+      const uint32_t lo = even ? own : got, hi = even ? got : own;      // of lanes 2n, 2n + 1
+      d32[0] = prmt(lo, hi, 0x5410u);
+      d32[8] = prmt(lo, hi, 0x7632u);
+    }
   }
 }
 
