@@ -13,15 +13,16 @@ namespace {
 __device__ int g_write_status;
 
 // ---------------------------------------------------------------- KV write
-// A warp takes two pairs of heads of one token (H of q, Hk of k, Hk of v), a
-// half-warp per head, so that the token's position, page and rotation row are
-// looked up once and eight loads a lane are in flight together.  Lane s of a half holds
+// A warp takes up to four heads of one kind (q, k or v) of one token, a half-warp
+// per head: what differs between the kinds is uniform in the warp, the token's
+// position, page and rotation row are looked up once, and eight loads a lane are
+// in flight together.  Lane s of a half holds
 // elements 2s, 2s + 1 of each 32-block: the RoPE partners i, i + 64 and the terms
 // that head_kernel (r4q_head_norm_rope) adds in one lane are in one lane here too,
 // and a butterfly over the half finishes the sum of squares in its order.  Norm
 // and rotation equal that kernel's to the bit, so a paged cache holds the bytes
-// that the contiguous one would.  Bound: issue slots (a warp per head with the
-// loads a lane-strided 2 bytes took 184 instructions a head).
+// that the contiguous one would.  Bound: issue slots (a warp per head took 184
+// instructions a head, mixed kinds in a warp 136).
 constexpr int kPairs = 2;
 constexpr int kHeads = 2 * kPairs;
 struct WriteArgs {
@@ -34,7 +35,7 @@ struct WriteArgs {
   PagedView c;
   const int* rows;
   const long long* pos;
-  int M, H, groups;                // groups of kHeads heads per token
+  int M, H, groups, q_groups, k_groups;   // groups of kHeads heads per token: q's, then k's, then v's
   FastDiv by_groups, by_page;
   float eps;
   int flags;
@@ -67,26 +68,28 @@ __device__ __forceinline__ float2 half2_of(uint32_t u) { return __half22float2(u
 __global__ void __launch_bounds__(256) paged_write_kernel(const WriteArgs a) {
   const int lane = threadIdx.x & 31, sl = lane & 15, half = lane >> 4;
   const int w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int m = a.by_groups.div(w), nh = a.H + 2 * a.c.Hk;
+  const int m = a.by_groups.div(w);
   if (m >= a.M) return;
   pdl_wait_trigger();
-  const int h0 = (w - m * a.groups) * kHeads;
+  int g = w - m * a.groups;
+  const bool is_q = g < a.q_groups, is_v = g >= a.q_groups + a.k_groups;
+  g -= is_q ? 0 : is_v ? a.q_groups + a.k_groups : a.q_groups;
+  const int h0 = g * kHeads, n = (is_q ? a.H : a.c.Hk) - h0;        // this warp: heads h0 .. of the kind, n left
   const long long pos = a.pos[m];
   const int row = a.rows ? a.rows[m] : m;
+  const int at = (h0 + half) * kHeadDim + 2 * sl;                   // this lane's first element in the token's row
+  const uint32_t* src = reinterpret_cast<const uint32_t*>(
+      (is_q ? a.q + m * a.ldq : is_v ? a.v + m * a.ldv : a.k + m * a.ldk) + at);
   uint32_t x32[kPairs][4];                           // before the position's lookups: independent of them
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) {
-    const int h = h0 + 2 * i + half;
-    const __half* src = h < a.H            ? a.q + m * a.ldq + (long)h * kHeadDim
-                        : h < a.H + a.c.Hk ? a.k + m * a.ldk + (long)(h - a.H) * kHeadDim
-                                           : a.v + m * a.ldv + (long)(h - a.H - a.c.Hk) * kHeadDim;
+  for (int i = 0; i < kPairs; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x32[i][j] = h < nh ? reinterpret_cast<const uint32_t*>(src)[sl + 16 * j] : 0u;
-  }
+    for (int j = 0; j < 4; ++j) x32[i][j] = 2 * i + half < n ? src[i * kHeadDim + 16 * j] : 0u;
   if (pos < 0) return;
-  const bool norm = a.flags & R4Q_HEAD_NORM, rope = a.flags & R4Q_HEAD_ROPE, full = a.flags & R4Q_KV_FULL_RANGE;
+  const bool norm = (a.flags & R4Q_HEAD_NORM) && !is_v, rope = (a.flags & R4Q_HEAD_ROPE) && !is_v;
+  const bool full = a.flags & R4Q_KV_FULL_RANGE;
   bool ok = row >= 0 && row < a.c.seqs && pos < (long long)a.c.max_blocks * a.c.page;
-  if (ok && rope) ok = pos < a.tab_rows;
+  if (ok && (a.flags & R4Q_HEAD_ROPE)) ok = pos < a.tab_rows;   // of a token, all heads or none
   int pg = 0, in_page = 0;
   float2 c[2] = {{1.f, 1.f}, {1.f, 1.f}}, s[2] = {{0.f, 0.f}, {0.f, 0.f}};
   if (ok) {
@@ -105,12 +108,20 @@ __global__ void __launch_bounds__(256) paged_write_kernel(const WriteArgs a) {
     if (lane == 0) atomicOr(&g_write_status, kPagedBadPage);
     return;
   }
+  uint32_t w32[4];
+  if (norm)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w32[j] = reinterpret_cast<const uint32_t*>(is_q ? a.qw : a.kw)[sl + 16 * j];
+  __half* out = is_q ? a.q_out + m * a.ldqo : !is_v && a.k_out ? a.k_out + m * a.ldko : nullptr;
+  uint32_t* o32 = reinterpret_cast<uint32_t*>(out + at);
+  const long head_bytes = (long)a.c.page * kHeadDim;
+  uint8_t* page = (is_v ? a.c.v + pg * a.c.v_stride : a.c.k + pg * a.c.k_stride) + (h0 + half) * head_bytes +
+                  in_page * kHeadDim;
+  const float* scale = is_v ? a.c.v_scale : a.c.k_scale;
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) {
-    const int h = h0 + 2 * i + half;
-    if (h0 + 2 * i >= nh) break;                     // uniform; from here on the halves stay together
-    const bool in = h < nh, is_q = h < a.H, is_v = h >= a.H + a.c.Hk;
-    const int kh = is_q ? 0 : is_v ? h - a.H - a.c.Hk : h - a.H;
+    if (2 * i >= n) break;                           // uniform
+    const bool in = 2 * i + half < n;
     float v[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -118,60 +129,49 @@ __global__ void __launch_bounds__(256) paged_write_kernel(const WriteArgs a) {
       v[2 * j] = f.x;
       v[2 * j + 1] = f.y;
     }
-    if (h0 + 2 * i < a.H + a.c.Hk) {                 // a q or k head among the two
-      if (norm) {
-        float s0 = 0.f, s1 = 0.f;
+    if (norm) {
+      float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s0 += v[2 * j] * v[2 * j];
-          s1 += v[2 * j + 1] * v[2 * j + 1];
-        }
-#pragma unroll
-        for (int d = 8; d > 0; d >>= 1) {
-          s0 += __shfl_xor_sync(0xffffffffu, s0, d);
-          s1 += __shfl_xor_sync(0xffffffffu, s1, d);
-        }
-        const float rrms = rsqrtf((s0 + s1) / (float)kHeadDim + a.eps);
-        const uint32_t* w32 = reinterpret_cast<const uint32_t*>(is_q ? a.qw : a.kw);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = half2_of(w32[sl + 16 * j]);
-          v[2 * j] = is_v ? v[2 * j] : v[2 * j] * rrms * f.x;
-          v[2 * j + 1] = is_v ? v[2 * j + 1] : v[2 * j + 1] * rrms * f.y;
-        }
+      for (int j = 0; j < 4; ++j) {
+        s0 += v[2 * j] * v[2 * j];
+        s1 += v[2 * j + 1] * v[2 * j + 1];
       }
-      if (rope && !is_v) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float e0 = v[2 * j], o0 = v[2 * j + 4], e1 = v[2 * j + 1], o1 = v[2 * j + 5];
-          v[2 * j] = e0 * c[j].x - o0 * s[j].x;
-          v[2 * j + 4] = o0 * c[j].x + e0 * s[j].x;
-          v[2 * j + 1] = e1 * c[j].y - o1 * s[j].y;
-          v[2 * j + 5] = o1 * c[j].y + e1 * s[j].y;
-        }
+      for (int d = 8; d > 0; d >>= 1) {
+        s0 += __shfl_xor_sync(0xffffffffu, s0, d);
+        s1 += __shfl_xor_sync(0xffffffffu, s1, d);
       }
-      __half* out = is_q ? a.q_out + m * a.ldqo + (long)h * kHeadDim
-                         : !is_v && a.k_out ? a.k_out + m * a.ldko + (long)kh * kHeadDim : nullptr;
-      if (in && out)
+      const float rrms = rsqrtf((s0 + s1) / (float)kHeadDim + a.eps);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          reinterpret_cast<uint32_t*>(out)[sl + 16 * j] = h2_as_u32(__floats2half2_rn(v[2 * j], v[2 * j + 1]));
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = half2_of(w32[j]);
+        v[2 * j] = v[2 * j] * rrms * f.x;
+        v[2 * j + 1] = v[2 * j + 1] * rrms * f.y;
+      }
     }
-    if (h0 + 2 * i + 1 < a.H) continue;              // two q heads
+    if (rope)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float e0 = v[2 * j], o0 = v[2 * j + 4], e1 = v[2 * j + 1], o1 = v[2 * j + 5];
+        v[2 * j] = e0 * c[j].x - o0 * s[j].x;
+        v[2 * j + 4] = o0 * c[j].x + e0 * s[j].x;
+        v[2 * j + 1] = e1 * c[j].y - o1 * s[j].y;
+        v[2 * j + 5] = o1 * c[j].y + e1 * s[j].y;
+      }
+    if (out && in)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        o32[i * kHeadDim + 16 * j] = h2_as_u32(__floats2half2_rn(v[2 * j], v[2 * j + 1]));
+    if (is_q) continue;
     // a lane has the codes of elements 2s, 2s + 1 of four 32-blocks: even lanes
     // store four bytes of blocks 0 and 1 with their neighbour's, odd lanes of 2 and 3
-    const float* scale = is_v ? a.c.v_scale : a.c.k_scale;
-    uint32_t e01 = 0, e23 = 0;
-    if (in && !is_q) {
-      e01 = encode2(v[0], v[1], scale, kh, full) | encode2(v[2], v[3], scale, kh, full) << 16;
-      e23 = encode2(v[4], v[5], scale, kh, full) | encode2(v[6], v[7], scale, kh, full) << 16;
-    }
+    const int kh = min(h0 + 2 * i + half, a.c.Hk - 1);
+    const uint32_t e01 = encode2(v[0], v[1], scale, kh, full) | encode2(v[2], v[3], scale, kh, full) << 16;
+    const uint32_t e23 = encode2(v[4], v[5], scale, kh, full) | encode2(v[6], v[7], scale, kh, full) << 16;
     const bool even = !(lane & 1);
     const uint32_t own = even ? e01 : e23, got = __shfl_xor_sync(0xffffffffu, even ? e23 : e01, 1);
-    if (in && !is_q) {
-      uint8_t* dst = (is_v ? a.c.v + pg * a.c.v_stride : a.c.k + pg * a.c.k_stride) +
-                     ((long)kh * a.c.page + in_page) * kHeadDim;
-      uint32_t* d32 = reinterpret_cast<uint32_t*>(dst) + (even ? 0 : 16) + (sl >> 1);
+    if (in) {
+      uint32_t* d32 = reinterpret_cast<uint32_t*>(page + 2 * i * head_bytes) + (even ? 0 : 16) + (sl >> 1);
       const uint32_t lo = even ? own : got, hi = even ? got : own;      // of lanes 2n, 2n + 1
       d32[0] = prmt(lo, hi, 0x5410u);
       d32[8] = prmt(lo, hi, 0x7632u);
@@ -279,7 +279,9 @@ extern "C" int r4q_paged_kv_write(const void* q, long ldq, const void* k, long l
   a.q_out = (__half*)q_out; a.k_out = (__half*)k_out; a.ldqo = ldqo; a.ldko = ldko;
   a.rows = rows; a.pos = pos;
   a.M = M; a.H = has_q ? H : 0; a.eps = eps; a.flags = flags;
-  a.groups = (a.H + 2 * a.c.Hk + kHeads - 1) / kHeads;
+  a.q_groups = (a.H + kHeads - 1) / kHeads;
+  a.k_groups = (a.c.Hk + kHeads - 1) / kHeads;
+  a.groups = a.q_groups + 2 * a.k_groups;
   a.by_groups = fast_div(a.groups);
   a.by_page = fast_div(a.c.page);
   const long warps = (long)M * a.groups;
