@@ -260,7 +260,7 @@ enum { R4Q_KV_FULL_RANGE = 8 };
  * the largest values near 448.
  * A token with pos[m] < 0 is padding: nothing of it is written.  A row,
  * position, page or table row out of range writes nothing and is reported by
- * r4q_paged_status.  Two tokens of one call must not name one position.
+ * r4q_kernel_status.  Two tokens of one call must not name one position.
  * 16-byte aligned pointers, row strides in multiples of 8 elements. */
 int r4q_paged_kv_write(const void* q, long ldq, const void* k, long ldk, const void* v, long ldv,
                        const void* q_norm_w, const void* k_norm_w, const void* cos_tab, const void* sin_tab,
@@ -273,7 +273,7 @@ int r4q_paged_kv_write(const void* q, long ldq, const void* k, long ldk, const v
  * sums, fp16 out, R4Q_ATTN_FWHT, zeros for an empty sequence).  B <= cache->seqs
  * rows; seq_lens int64 [B], device; any H that is a multiple of Hk.  A page id
  * outside the pool reads as zeros, a length beyond max_blocks * page is cut;
- * both are reported by r4q_paged_status.  Bytes of a page behind the sequence
+ * both are reported by r4q_kernel_status.  Bytes of a page behind the sequence
  * may hold anything.  workspace (16-byte aligned, of the size that
  * r4q_paged_flash_decode_workspace_bytes gives; may be 0, then NULL) needs no
  * initialisation and keeps nothing between calls; calls that may run at once
@@ -282,10 +282,12 @@ size_t r4q_paged_flash_decode_workspace_bytes(int B, int H, int Hk, int page, in
 int r4q_paged_flash_decode(const void* q, long ldq, const r4q_paged_cache* cache, const long long* seq_lens, void* o,
                            long ldo, int B, int H, int flags, void* workspace, size_t ws_bytes, void* stream);
 
-/* R4Q_ERR_PAGE / R4Q_ERR_TIMEOUT if a paged kernel of the current device met an
- * id out of range / gave up a wait since the last clear, else R4Q_OK.
+/* R4Q_ERR_PAGE if a paged kernel of the current device met an id out of range
+ * since the last clear, R4Q_ERR_TIMEOUT if a bounded wait of the paged attention
+ * or of r4q_token_logprobs gave up (those outputs are not valid), else R4Q_OK.
+ * Their status words live in the library, one per device: no workspace to pass.
  * Synchronises the device. */
-int r4q_paged_status(int clear);
+int r4q_kernel_status(int clear);
 
 /* pool[l][dst[i]] = pool[l][src[i]] for every i < n and every l < outer: pages of
  * page_bytes, page_stride apart, in `outer` pools (layers, K and V)

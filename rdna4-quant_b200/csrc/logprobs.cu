@@ -1,46 +1,93 @@
 // Likelihoods of given tokens: log softmax at the token, its rank, the entropy
 // of the row and its k most likely ids, in one pass over the logits.
 //
-//   m = max x,  S = sum e^(x - m),  A = sum e^(x - m) (x - m)
-//   logprob = (x_t - m) - log S,    entropy = log S - A / S
+//   m = max x,  t = (x - m) log2(e),  S = sum 2^t,  A = sum 2^t t
+//   logprob = (x_t - m) - ln2 log2 S,    entropy = ln2 (log2 S - A / S)
 //
-// (m, S, A) of parts join like a softmax's: with M = max m and f = e^(m - M),
-// S <- sum f S and A <- sum f (A + S (m - M)).  Ids are ordered by one 64-bit
-// key (value, lowest id first), so every selection has one right answer.
+// (m, S, A) of parts join like a softmax's: with M = max m, d = (m - M) log2(e)
+// and f = 2^d, S <- sum f S and A <- sum f (A + S d).  Ids are ordered by one
+// 64-bit key (value, lowest id first), so every selection has one right answer.
 //
-// Bound: HBM, each logit read once.  A cluster of C CTAs shares a row (C = 1 for
-// many rows; up to 8 for few, so that a single row of a large vocabulary is
-// spread over the SMs); a thread keeps four 16-byte loads in flight, takes their
-// maximum on packed pairs, and rescales its running sums only when that moved.
+// Bound: HBM, each logit read once, if the issue slots allow: 11.6 logits a clock
+// and SM at the measured bandwidth, of some five instructions each.  So maxima
+// are taken on packed pairs, the sums with two-wide fp32 instructions, the
+// running sums are rescaled only when the maximum moved, and f16 logits need one
+// multiply-add for t: 2^t is taken from x log2(e) - M with M the rounded
+// m log2(e), whose rounding (at most 2^-8) the thread takes out of its sums once.
+// (bf16 and fp32 logits may be so large that it would not be small: subtract first.)
+// A cluster of C CTAs shares a row (C = 1 for many rows; up to 8 for few, so that
+// a single row of a large vocabulary is spread over the SMs); CTAs are small, so
+// that others stream while one selects.  Every warp streams its own 2 KB chunks
+// through a ring in shared memory by bulk copies, two ahead: loads ahead in
+// registers cost occupancy or spills (2048 x 151936 f16, top 5: 294 us with a chunk
+// ahead in registers, 199 us without).
 //
 // Top k.  While it streams, every thread keeps its largest value and the place
 // of the chunk that had it, i.e. an upper and a lower bound of its largest key.
 // The k-th largest of the lower bounds of disjoint groups of elements is a lower
-// bound tau of the k-th largest key, and a close one: of 128 groups of four
-// threads, about k (1 + k / 256) elements reach it.  Only groups whose upper
-// bound reaches tau are read again (k of 128, from L2, unless values tie), and
-// what reaches tau, some k elements, goes into sorted warp lists of 32 that bound
-// the count whatever the values are (ties, masks, sorted rows).  Ranks among
-// the lists' keys then give the CTA's order, and sorted lists of CTAs merge.
+// bound tau of the k-th largest key, and a close one: of 128 groups of threads,
+// about k (1 + k / 256) elements reach it.  Only the elements of threads whose
+// upper bound reaches tau are read again (some k threads, from L2, unless values
+// tie), by a warp per thread; what reaches tau goes into sorted warp lists of 32,
+// which bound the count whatever the values are (ties, masks, sorted rows).  Ranks
+// among the lists' keys then give the CTA's order, and sorted lists of CTAs merge.
 #include <cuda_bf16.h>
 
+#include <mutex>
+#include <type_traits>
+
+#include "paged.cuh"
 #include "r4q_common.cuh"
+#include "tma_dev.cuh"
 
 namespace r4q {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
+constexpr int kResident = 4;              // CTAs per SM that the registers allow
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
-constexpr int kGroups = kThreads / 4;     // of four neighbouring threads
+constexpr int kGroups = 128;              // of neighbouring threads
+constexpr int kGroupLanes = kThreads / kGroups;
 constexpr int kMaxCluster = 8;
-constexpr int kUnroll = 4;                // 16-byte loads in flight per thread
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kUnroll = 4;                // 16-byte words of a lane in a chunk
+constexpr int kChunk = 32 * kUnroll;      // words of a warp's chunk, 2 KB
+constexpr int kStages = 2;                // chunks of a warp's ring
+constexpr int kPolls = 1 << 22;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kTiny = -150.f;           // 2^kTiny is 0 in fp32: also stands for log2 0, where 0 * -inf would be NaN
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// two fp32 operations an instruction
+struct F2 {
+  uint64_t v;
+  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ explicit F2(uint64_t u) : v(u) {}
+  __device__ __forceinline__ float2 get() const {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+  }
+};
+__device__ __forceinline__ F2 add(F2 a, F2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
+  return F2(d);
+}
+__device__ __forceinline__ F2 mul(F2 a, F2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
+  return F2(d);
+}
+__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return F2(d);
 }
 
 // order of floats as unsigned integers; NaN is the lowest, -0 equals +0
@@ -58,8 +105,8 @@ __device__ __forceinline__ float value_of(uint64_t key) {
   return o == 0u ? __int_as_float(0x7fc00000) : __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
 }
 
-// A type's 16-byte word: its floats, the largest of four words (NaN if there
-// is one; `skip` passes over NaN), and the word of single elements.
+// A type's 16-byte word: its floats, its largest and the largest of four words
+// (NaN if there is one), and how single elements are read.
 template <typename X> struct Vec;
 template <> struct Vec<__half> {
   static constexpr int n = 8;
@@ -86,9 +133,20 @@ template <> struct Vec<__half> {
     m.w = mx(mx(u[0].w, u[1].w), mx(u[2].w, u[3].w));
     return most(m);
   }
+  // how many elements of four words exceed the words' thresholds (a pair of one value each)
+  static __device__ __forceinline__ int above(const uint4 (&u)[4], const uint32_t (&th)[4]) {
+    __half2 a = __float2half2_rn(0.f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __half2 h = u32_as_h2(th[j]);
+      a = __hadd2(a, __hadd2(__hadd2(__hgt2(u32_as_h2(u[j].x), h), __hgt2(u32_as_h2(u[j].y), h)),
+                             __hadd2(__hgt2(u32_as_h2(u[j].z), h), __hgt2(u32_as_h2(u[j].w), h))));
+    }
+    return __half2int_rn(__hadd(__low2half(a), __high2half(a)));
+  }
   static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
   static __device__ __forceinline__ uint32_t bits(const __half* p) { return __half_as_ushort(*p); }
-  static constexpr uint32_t kNegInf = 0xfc00u;
+  static constexpr uint32_t kNegInf = 0xfc00u, kSign = 0x8000u, kPair = 0x10001u;
 };
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int n = 8;
@@ -117,9 +175,20 @@ template <> struct Vec<__nv_bfloat16> {
     m.w = mx(mx(u[0].w, u[1].w), mx(u[2].w, u[3].w));
     return most(m);
   }
+  static __device__ __forceinline__ int above(const uint4 (&u)[4], const uint32_t (&th)[4]) {
+    auto b2 = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+    __nv_bfloat162 a = __float2bfloat162_rn(0.f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __nv_bfloat162 h = b2(th[j]);
+      a = __hadd2(a, __hadd2(__hadd2(__hgt2(b2(u[j].x), h), __hgt2(b2(u[j].y), h)),
+                             __hadd2(__hgt2(b2(u[j].z), h), __hgt2(b2(u[j].w), h))));
+    }
+    return (int)(__low2float(a) + __high2float(a));
+  }
   static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
   static __device__ __forceinline__ uint32_t bits(const __nv_bfloat16* p) { return __bfloat16_as_ushort(*p); }
-  static constexpr uint32_t kNegInf = 0xff80u;
+  static constexpr uint32_t kNegInf = 0xff80u, kSign = 0x8000u, kPair = 0x10001u;
 };
 template <> struct Vec<float> {
   static constexpr int n = 4;
@@ -140,9 +209,19 @@ template <> struct Vec<float> {
   static __device__ __forceinline__ float most4(const uint4 (&u)[4]) {
     return mx(mx(most(u[0]), most(u[1])), mx(most(u[2]), most(u[3])));
   }
+  static __device__ __forceinline__ int above(const uint4 (&u)[4], const uint32_t (&th)[4]) {
+    int a = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float h = __uint_as_float(th[j]);
+      a += (__uint_as_float(u[j].x) > h) + (__uint_as_float(u[j].y) > h) + (__uint_as_float(u[j].z) > h) +
+           (__uint_as_float(u[j].w) > h);
+    }
+    return a;
+  }
   static __device__ __forceinline__ float one(const float* p) { return *p; }
   static __device__ __forceinline__ uint32_t bits(const float* p) { return __float_as_uint(*p); }
-  static constexpr uint32_t kNegInf = 0xff800000u;
+  static constexpr uint32_t kNegInf = 0xff800000u, kSign = 0x80000000u, kPair = 1u;
 };
 
 // A row as 16-byte words of the memory it lies in: word i holds elements
@@ -151,15 +230,17 @@ template <> struct Vec<float> {
 template <typename X>
 struct Row {
   const X* x;
-  int V, head, words;
+  int V, head, words, lo, hi;              // words lo .. hi are the row's entirely
   __device__ __forceinline__ Row(const X* p, int V_) : x(p), V(V_) {
     head = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(X));
     words = (head + V + Vec<X>::n - 1) / Vec<X>::n;
+    lo = head ? 1 : 0;
+    hi = (head + V) / Vec<X>::n - 1;
   }
   __device__ __forceinline__ int first(int i) const { return i * Vec<X>::n - head; }   // element
   __device__ __forceinline__ uint4 load(int i) const {
     const int e = first(i);
-    if (i < words && e >= 0 && e + Vec<X>::n <= V) return *reinterpret_cast<const uint4*>(x + e);
+    if (i >= lo && i <= hi) return *reinterpret_cast<const uint4*>(x + e);
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < Vec<X>::n; ++j) {
@@ -168,6 +249,9 @@ struct Row {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
+  // whether the chunk of words from i on is the row's entirely, i.e. may be copied in bulk
+  __device__ __forceinline__ bool bulk(int i) const { return i >= lo && i + kChunk - 1 <= hi; }
+  __device__ __forceinline__ const void* at(int i) const { return x - head + (long)i * Vec<X>::n; }
 };
 
 struct Sums {
@@ -175,7 +259,7 @@ struct Sums {
   __device__ __forceinline__ void join(float m2, float S2, float A2) {
     const float M = fmaxf(m, m2);
     if (M == -INFINITY) return;
-    const float d = fmaxf(m - M, -1e4f), d2 = fmaxf(m2 - M, -1e4f), f = ex2(d * kLog2e), f2 = ex2(d2 * kLog2e);
+    const float d = fmaxf((m - M) * kLog2e, kTiny), d2 = fmaxf((m2 - M) * kLog2e, kTiny), f = ex2(d), f2 = ex2(d2);
     A = f * (A + S * d) + f2 * (A2 + S2 * d2);
     S = f * S + f2 * S2;
     m = M;
@@ -186,10 +270,12 @@ struct Shared {
   alignas(16) uint64_t group[kGroups];   // lower bound of the largest key of each group of this CTA
   uint64_t list[kWarps * kMaxTop];       // collected keys
   uint64_t top[kMaxTop];                 // this CTA's k best
+  uint64_t bars[kWarps * kStages];
   float m[kWarps], S[kWarps], A[kWarps];
   int before[kWarps], nan[kWarps];
+  unsigned short open[kThreads];         // threads whose elements are read again
   uint64_t tau;
-  int n_list;
+  int n_open, n_list;
   float cm, cS, cA;                      // this CTA's sums
   int cbefore, cnan;
 };
@@ -240,30 +326,100 @@ __device__ __forceinline__ uint64_t merge(uint64_t a, uint64_t b, int lane) {
   return v;
 }
 
+__device__ int g_logprob_status;         // a bounded wait gave up
+
+__device__ __forceinline__ bool wait_full(uint64_t* bar, unsigned parity) {
+  const uint32_t b = smem_u32(bar);
+  for (int i = 0; i < kPolls; ++i) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+                 " selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(b), "r"(parity) : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ void copy_chunk(void* dst, const void* src, uint64_t* bar) {
+  mbar_expect_tx(bar, kChunk * 16);
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)), "l"(src), "r"(kChunk * 16), "r"(smem_u32(bar)) : "memory");
+}
+
 template <typename X>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, kResident)
     logprobs_kernel(const X* __restrict__ logits, long ld, const long long* __restrict__ tokens, int V, int k,
                     float* logprob, long long* rank_out, float* entropy, long long* top_ids, float* top_lp) {
   constexpr int n = Vec<X>::n;
   __shared__ Shared sh;
+  extern __shared__ __align__(16) uint4 ring_mem[];    // [warp][stage][kChunk]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = gridDim.x, cta = blockIdx.x;
   const long row = blockIdx.y;
-  pdl_wait_trigger();
   const Row<X> r(logits + row * ld, V);
+  if (lane == 0) {
+#pragma unroll
+    for (int j = 0; j < kStages; ++j) mbar_init(&sh.bars[warp * kStages + j], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
+  pdl_wait_trigger();
   const long long tok = tokens ? tokens[row] : -1;
   const bool has_t = tok >= 0 && tok < V;
   const int t = has_t ? (int)tok : -1;
   const float xt = has_t ? Vec<X>::one(r.x + t) : INFINITY;
+  // what precedes the token: values above xt, and with a lower id those equal to
+  // it, i.e. above the next lower value
+  const uint32_t tb = has_t ? Vec<X>::bits(r.x + t) : 0u;
+  const uint32_t above_t = tb * Vec<X>::kPair;
+  const uint32_t from_t = ((tb & ~Vec<X>::kSign) == 0 ? Vec<X>::kSign | 1u : tb & Vec<X>::kSign ? tb + 1 : tb - 1) *
+                          Vec<X>::kPair;
+  const bool plain_t = fabsf(xt) < INFINITY;
 
-  // ---- one pass: this CTA's words cta * kThreads + tid, strided by C * kThreads
-  Sums s;
+  // ---- one pass: chunks of the row, dealt to the warps of the cluster in turn
+  constexpr bool kFused = std::is_same<X, __half>::value;    // t in one multiply-add
+  const F2 l2e(kLog2e, kLog2e);
+  F2 S2(0.f, 0.f), A2(0.f, 0.f), shift(0.f, 0.f);
+  float most = -INFINITY, M = 0.f;           // running maximum; what t is relative to: m, or m log2(e) rounded
   float best = -INFINITY;
   int best_w = -1, before = 0, nan = 0;      // best_w: first word of the chunk with the thread's largest value
-  const int stride = C * kThreads;
-  for (int i = cta * kThreads + tid; i < r.words; i += kUnroll * stride) {
-    uint4 u[kUnroll];
+  const int stride = C * kWarps * kChunk, begin = (cta * kWarps + warp) * kChunk;
+  uint4* ring = ring_mem + warp * kStages * kChunk;
+  uint64_t* bars = sh.bars + warp * kStages;
+  if (lane == 0)
 #pragma unroll
-    for (int j = 0; j < kUnroll; ++j) u[j] = r.load(i + j * stride);
+    for (int j = 0; j < kStages; ++j)
+      if (begin + j * stride < r.words && r.bulk(begin + j * stride))
+        copy_chunk(ring + j * kChunk, r.at(begin + j * stride), &bars[j]);
+  int stage = 0;
+  unsigned parity = 0;                       // bit j: of stage j
+  for (int base = begin; base < r.words; base += stride) {
+    const int i = base + lane;               // this lane's words: i, i + 32, ..
+    uint4 u[kUnroll];
+    if (r.bulk(base)) {
+      if (!wait_full(&bars[stage], parity >> stage & 1)) {
+        // the copies in flight get their time once more; the row's results are void
+        for (int j = 1; j < kStages; ++j) {
+          const int s2 = (stage + j) % kStages, at = base + j * stride;
+          if (at < r.words && r.bulk(at)) wait_full(&bars[s2], parity >> s2 & 1);
+        }
+        if (lane == 0) atomicOr(&g_logprob_status, kPagedTimeout);
+        nan = 1;
+        break;
+      }
+      parity ^= 1u << stage;
+#pragma unroll
+      for (int j = 0; j < kUnroll; ++j) u[j] = ring[stage * kChunk + lane + 32 * j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < kUnroll; ++j) u[j] = r.load(i + 32 * j);
+    }
+    __syncwarp();
+    if (lane == 0) {                         // the stage is in registers: its next chunk may come
+      const int at = base + kStages * stride;
+      if (at < r.words && r.bulk(at)) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        copy_chunk(ring + stage * kChunk, r.at(at), &bars[stage]);
+      }
+    }
+    stage = stage + 1 == kStages ? 0 : stage + 1;
     float c = Vec<X>::most4(u);
     if (c != c) {                            // NaN: the row is none; the order goes on without it
       nan = 1;
@@ -280,52 +436,81 @@ __global__ void __launch_bounds__(kThreads, 2)
       best = c;
       best_w = i;
     }
-    if (c > s.m) {
-      const float d = fmaxf(s.m - c, -1e4f), f = ex2(d * kLog2e);
-      s.A = f * (s.A + s.S * d);
-      s.S *= f;
-      s.m = c;
+    if (c > most) {
+      const float to = kFused ? c * kLog2e : c;
+      const float d = most == -INFINITY ? kTiny : fmaxf(kFused ? M - to : (M - to) * kLog2e, kTiny), f = ex2(d);
+      A2 = mul(F2(f, f), fma(S2, F2(d, d), A2));
+      S2 = mul(F2(f, f), S2);
+      most = c;
+      M = to;
+      shift = F2(-to, -to);
     }
-    const float m = s.m == -INFINITY ? 0.f : s.m;
-    const bool count = c >= xt || xt != xt;
+    const bool count = has_t && (c >= xt || xt != xt);
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
       float x[n];
       Vec<X>::get(u[j], x);
 #pragma unroll
-      for (int q = 0; q < n; ++q) {
-        const float d = fmaxf(x[q] - m, -1e4f), e = ex2(d * kLog2e);   // -inf: no 0 * inf
-        s.S += e;
-        s.A = fmaf(e, d, s.A);
+      for (int q = 0; q < n; q += 2) {
+        const F2 two(x[q], x[q + 1]);
+        float2 t2 = (kFused ? fma(two, l2e, shift) : mul(add(two, shift), l2e)).get();
+        t2.x = fmaxf(t2.x, kTiny);
+        t2.y = fmaxf(t2.y, kTiny);
+        const F2 e(ex2(t2.x), ex2(t2.y));
+        S2 = add(S2, e);
+        A2 = fma(e, F2(t2.x, t2.y), A2);
       }
-      if (count) {                           // what precedes the token
-        const int e0 = r.first(i + j * stride);
+    }
+    if (count) {
+      uint32_t th[kUnroll];
+      bool has = !plain_t;
 #pragma unroll
-        for (int q = 0; q < n; ++q) {
-          const unsigned e = (unsigned)(e0 + q);
-          if (xt == xt) before += x[q] > xt || (x[q] == xt && e < (unsigned)t);
-          else before += e < (unsigned)V && (x[q] == x[q] || e < (unsigned)t);
+      for (int j = 0; j < kUnroll; ++j) {
+        const int e0 = r.first(i + 32 * j);
+        th[j] = e0 < t ? from_t : above_t;
+        has |= (unsigned)(t - e0) < (unsigned)n;
+      }
+      if (!has) {
+        before += Vec<X>::above(u, th);
+      } else {                               // the token's own chunk; a token of no finite value
+#pragma unroll
+        for (int j = 0; j < kUnroll; ++j) {
+          const int e0 = r.first(i + 32 * j);
+          float x[n];
+          Vec<X>::get(u[j], x);
+#pragma unroll
+          for (int q = 0; q < n; ++q) {
+            const unsigned e = (unsigned)(e0 + q);
+            before += xt == xt ? x[q] > xt || (x[q] == xt && e < (unsigned)t)
+                               : e < (unsigned)V && (x[q] == x[q] || e < (unsigned)t);
+          }
         }
       }
     }
   }
+  Sums s;
+  s.m = most;
+  {
+    const float2 a = S2.get(), b = A2.get();
+    const float off = kFused && most > -INFINITY && most < INFINITY ? fmaf(most, kLog2e, -M) : 0.f, f = ex2(-off);
+    s.S = (a.x + a.y) * f;
+    s.A = (b.x + b.y - off * (a.x + a.y)) * f;
+  }
 
-  // ---- the CTA's sums, and bounds of the largest key of each group of four threads
+  // ---- bounds of the largest key of the thread, and the CTA's sums
   uint64_t upper = 0, lower = 0;
   if (best_w >= 0) {
     upper = key_of(best, max(0, r.first(best_w)));
-    // of its chunk, the last element of the row
-    const int w = best_w + min(kUnroll - 1, (r.words - 1 - best_w) / stride) * stride;
-    lower = key_of(best, min(V - 1, r.first(w) + n - 1));
+    lower = key_of(best, min(V - 1, r.first(best_w + 32 * (kUnroll - 1)) + n - 1));   // the chunk's last, or a later one
   }
+  // of the group; a value of -inf may stand for NaN alone, which comes after it: no bound
+  uint64_t bound = (uint32_t)(lower >> 32) > ordered(-INFINITY) ? lower : 0ull;
 #pragma unroll
-  for (int d = 1; d < 4; d <<= 1) {
-    const uint64_t o = __shfl_xor_sync(0xffffffffu, upper, d), p = __shfl_xor_sync(0xffffffffu, lower, d);
-    upper = o > upper ? o : upper;
-    lower = p > lower ? p : lower;
+  for (int d = 1; d < kGroupLanes; d <<= 1) {
+    const uint64_t o = __shfl_xor_sync(0xffffffffu, bound, d);
+    bound = o > bound ? o : bound;
   }
-  // -inf may stand for NaN alone, which comes after it: no bound
-  if (lane % 4 == 0) sh.group[tid >> 2] = (uint32_t)(lower >> 32) > ordered(-INFINITY) ? lower : 0ull;
+  if (lane % kGroupLanes == 0) sh.group[tid / kGroupLanes] = bound;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {
     s.join(__shfl_xor_sync(0xffffffffu, s.m, d), __shfl_xor_sync(0xffffffffu, s.S, d),
@@ -341,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     sh.nan[warp] = nan;
   }
   if (tid == 0) {
-    sh.n_list = 0;
+    sh.n_list = sh.n_open = 0;
     sh.tau = 0;
   }
   if (tid < kMaxTop) sh.top[tid] = 0;
@@ -386,21 +571,28 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     __syncthreads();
     const uint64_t tau = sh.tau;
+    const bool again = upper >= tau && begin + lane < r.words;            // no bound: every thread's
+    const unsigned who = __ballot_sync(0xffffffffu, again);
+    int at = 0;
+    if (lane == 0 && who) at = atomicAdd(&sh.n_open, __popc(who));        // in any order, like the lists below:
+    at = __shfl_sync(0xffffffffu, at, 0);                                 // the keys are ranked in the end
+    if (again) sh.open[at + __popc(who & ((1u << lane) - 1))] = (unsigned short)tid;
+    __syncthreads();
+    const int n_open = sh.n_open;
     const float tau_value = value_of(tau);
     uint64_t mine = 0;                                 // the warp's best so far, lane i the i-th
-    unsigned open = __ballot_sync(0xffffffffu, lane % 4 == 0 && upper >= tau);   // no bound: every group
-    for (; open; open &= open - 1) {                   // a group's words: four neighbours in each stride
-      const int first = cta * kThreads + warp * 32 + __ffs(open) - 1;
-      for (int base = 0; first + base * stride < r.words; base += 8) {   // 8 strides x 4 words at once
-        const int w = first + lane % 4 + (base + lane / 4) * stride;
+    for (int q = warp; q < n_open; q += kWarps) {      // a thread's words, a chunk per four lanes
+      const int who = sh.open[q], first = (cta * kWarps + (who >> 5)) * kChunk + (who & 31);
+      for (int base = 0; first + base * stride < r.words; base += 32 / kUnroll) {
+        const int w = first + (base + lane / kUnroll) * stride + 32 * (lane % kUnroll);
         const uint4 u = r.load(w);
         if (tau && !__any_sync(0xffffffffu, !(Vec<X>::most(u) < tau_value))) continue;
         float x[n];
         Vec<X>::get(u, x);
 #pragma unroll
-        for (int q = 0; q < n; ++q) {
-          const int e = r.first(w) + q;
-          const uint64_t key = w < r.words && e >= 0 && e < V ? key_of(x[q], e) : 0ull;
+        for (int j = 0; j < n; ++j) {
+          const int e = r.first(w) + j;
+          const uint64_t key = w < r.words && e >= 0 && e < V ? key_of(x[j], e) : 0ull;
           const uint64_t floor = __shfl_sync(0xffffffffu, mine, k - 1);
           unsigned in = __ballot_sync(0xffffffffu, key >= tau && key > floor);
           for (; in; in &= in - 1) insert(mine, __shfl_sync(0xffffffffu, key, __ffs(in) - 1), lane);
@@ -408,8 +600,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
     const unsigned have = __ballot_sync(0xffffffffu, lane < k && mine);
-    int at = 0;
-    if (lane == 0 && have) at = atomicAdd(&sh.n_list, __popc(have));   // in any order: the keys are ranked below
+    if (lane == 0 && have) at = atomicAdd(&sh.n_list, __popc(have));
     at = __shfl_sync(0xffffffffu, at, 0);
     if (have >> lane & 1) sh.list[at + lane] = mine;
     __syncthreads();
@@ -448,11 +639,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     const float m = __shfl_sync(0xffffffffu, c.m, 0), S = __shfl_sync(0xffffffffu, c.S, 0);
     const bool none = __shfl_sync(0xffffffffu, bad, 0) || isinf(m);
-    const float quiet = __int_as_float(0x7fc00000), logS = logf(S);
+    const float quiet = __int_as_float(0x7fc00000), logS = log2f(S);
     if (lane == 0) {
-      if (logprob) logprob[row] = none || !has_t ? quiet : xt - m - logS;
+      if (logprob) logprob[row] = none || !has_t ? quiet : xt - m - kLn2 * logS;
       if (rank_out) rank_out[row] = has_t ? b + 1 : 0;
-      if (entropy) entropy[row] = none ? quiet : logS - c.A / S;
+      if (entropy) entropy[row] = none ? quiet : kLn2 * (logS - c.A / S);
     }
     if (k > 0) {
       if (C > 1)
@@ -462,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int q = 0; q < d; ++q) list[q] = merge(list[q], list[q + d], lane);
       if (lane < k) {
         if (top_ids) top_ids[row * k + lane] = id_of(list[0]);
-        if (top_lp) top_lp[row * k + lane] = none ? quiet : value_of(list[0]) - m - logS;
+        if (top_lp) top_lp[row * k + lane] = none ? quiet : value_of(list[0]) - m - kLn2 * logS;
       }
     }
   }
@@ -472,14 +663,32 @@ __global__ void __launch_bounds__(kThreads, 2)
 template <typename X>
 int launch(const void* logits, long ld, const long long* tokens, int M, int V, int k, float* logprob, long long* rank,
            float* entropy, long long* top_ids, float* top_lp, cudaStream_t st) {
-  // CTAs per row: as many as keep one word per thread and the grid within two CTAs an SM
+  constexpr int kRing = kWarps * kStages * kChunk * 16;
+  static std::mutex mu;
+  static bool attr_done[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (dev >= 64 || !attr_done[dev]) {
+      const cudaError_t e =
+          cudaFuncSetAttribute(logprobs_kernel<X>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
+      if (e != cudaSuccess) {
+        cudaGetLastError();
+        return set_error(R4Q_ERR_CUDA, "logprobs_kernel: %s", cudaGetErrorString(e));
+      }
+      if (dev < 64) attr_done[dev] = true;
+    }
+  }
+  // CTAs per row: as many as keep one chunk per warp and the grid within one wave
   int C = kMaxCluster;
-  while (C > 1 && ((long)M * C > 2L * num_sms() || (long)(C / 2) * kThreads * Vec<X>::n >= V)) C >>= 1;
+  while (C > 1 && ((long)M * C > (long)kResident * num_sms() || (long)(C / 2) * kWarps * kChunk * Vec<X>::n >= V)) C >>= 1;
   for (int at = 0; at < M; at += 65535) {
     const int rows = M - at < 65535 ? M - at : 65535;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(C, rows);
     cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kRing;
     cfg.stream = st;
     cudaLaunchAttribute attrs[2];
     attrs[0].id = cudaLaunchAttributeClusterDimension;
@@ -504,6 +713,14 @@ int launch(const void* logits, long ld, const long long* tokens, int M, int V, i
 }
 
 }  // namespace
+
+cudaError_t logprob_status(int clear, int* word) {
+  const int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(word, g_logprob_status, sizeof(int));
+  if (e == cudaSuccess && *word && clear) e = cudaMemcpyToSymbol(g_logprob_status, &zero, sizeof(int));
+  return e;
+}
+
 }  // namespace r4q
 
 using namespace r4q;

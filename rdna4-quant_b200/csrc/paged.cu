@@ -1,6 +1,6 @@
 // Paged FP8 KV cache: new tokens into pages (with the per-head RMSNorm + RoPE
 // of q and k), page copies over all layers, block-table updates, and the
-// status word of the paged kernels.
+// status of the kernels that keep their status words in the library.
 #include <cstring>
 #include <vector>
 
@@ -357,21 +357,23 @@ extern "C" int r4q_kv_table_set(int* table, long ld, int rows, int cols, const i
   return R4Q_OK;
 }
 
-extern "C" int r4q_paged_status(int clear) {
-  int a = 0, b = 0;
+extern "C" int r4q_kernel_status(int clear) {
+  int a = 0, b = 0, c = 0;
   const int zero = 0;
   cudaError_t e = cudaDeviceSynchronize();
   if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&a, g_write_status, sizeof(int));
   if (e == cudaSuccess && a && clear) e = cudaMemcpyToSymbol(g_write_status, &zero, sizeof(int));
   if (e == cudaSuccess) e = paged_attn_status(clear, &b);
+  if (e == cudaSuccess) e = logprob_status(clear, &c);
   if (e != cudaSuccess) {
     cudaGetLastError();
-    return set_error(R4Q_ERR_CUDA, "paged_status: %s", cudaGetErrorString(e));
+    return set_error(R4Q_ERR_CUDA, "kernel_status: %s", cudaGetErrorString(e));
   }
   if ((a | b) & kPagedBadPage)
-    return set_error(R4Q_ERR_PAGE, "a paged %s met a row, position or page id outside the cache since the last check",
-                     a & kPagedBadPage ? "write" : "attention");
-  if ((a | b) & kPagedTimeout)
-    return set_error(R4Q_ERR_TIMEOUT, "a bounded wait of the paged attention gave up since the last check");
+    return set_error(R4Q_ERR_PAGE, "a paged %s met a row, position, length or page id outside the cache since the last "
+                     "check", a & kPagedBadPage ? "write" : "attention");
+  if ((b | c) & kPagedTimeout)
+    return set_error(R4Q_ERR_TIMEOUT, "a bounded wait of the %s kernel gave up since the last check: its outputs are "
+                     "not valid", b & kPagedTimeout ? "paged attention" : "likelihood");
   return R4Q_OK;
 }

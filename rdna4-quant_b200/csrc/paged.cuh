@@ -1,5 +1,5 @@
-// Shared by the paged-cache kernels: the checked view of r4q_paged_cache and
-// the status bits that r4q_paged_status reports.
+// Shared by the paged-cache and likelihood kernels: the checked view of
+// r4q_paged_cache and the status bits that r4q_kernel_status reports.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -37,7 +37,8 @@ struct PagedView {
 
 // Checks the caller's description and fills the view; `what` names the caller.
 int paged_view(const char* what, const r4q_paged_cache* c, PagedView* out);
-// Status word of the attention kernels (the device is idle).
+// Status words of the attention and the likelihood kernels (the device is idle).
 cudaError_t paged_attn_status(int clear, int* word);
+cudaError_t logprob_status(int clear, int* word);
 
 }  // namespace r4q

@@ -92,9 +92,9 @@ def check_status(dev: torch.device | int | None = None, clear: bool = True) -> N
         st = L.LIB.r4q_ws_status(None, 1 if clear else 0, None)
         if st != 0 and err is None:
             err = L.R4QError(st, "r4q_ws_status(noalloc scratch)", L.last_error())
-        st = L.LIB.r4q_paged_status(1 if clear else 0)
+        st = L.LIB.r4q_kernel_status(1 if clear else 0)
         if st != 0 and err is None:
-            err = L.R4QError(st, "r4q_paged_status", L.last_error())
+            err = L.R4QError(st, "r4q_kernel_status", L.last_error())
     if err is not None:
         raise err
 
