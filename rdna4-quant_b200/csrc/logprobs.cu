@@ -28,9 +28,11 @@
 // bound tau of the k-th largest key, and a close one: of 128 groups of threads,
 // about k (1 + k / 256) elements reach it.  Only the elements of threads whose
 // upper bound reaches tau are read again (some k threads, from L2, unless values
-// tie), by a warp per thread; what reaches tau goes into sorted warp lists of 32,
-// which bound the count whatever the values are (ties, masks, sorted rows).  Ranks
-// among the lists' keys then give the CTA's order, and sorted lists of CTAs merge.
+// tie), by the whole CTA at once, and what reaches tau is put into a list.  Should
+// that overflow (ties, masks, sorted rows), every warp goes through its own
+// threads' elements with a sorted list of its 32 best, which bounds the count
+// whatever the values are.  Ranks among the lists' keys then give the CTA's
+// order, and sorted lists of CTAs merge.
 #include <cuda_bf16.h>
 
 #include <mutex>
@@ -49,6 +51,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
 constexpr int kGroups = 128;              // of neighbouring threads
 constexpr int kGroupLanes = kThreads / kGroups;
+constexpr int kList = kWarps * kMaxTop;   // collected keys of a CTA
 constexpr int kMaxCluster = 8;
 constexpr int kUnroll = 4;                // 16-byte words of a lane in a chunk
 constexpr int kChunk = 32 * kUnroll;      // words of a warp's chunk, 2 KB
@@ -268,12 +271,12 @@ struct Sums {
 
 struct Shared {
   alignas(16) uint64_t group[kGroups];   // lower bound of the largest key of each group of this CTA
-  uint64_t list[kWarps * kMaxTop];       // collected keys
+  uint64_t list[kList];                  // collected keys
   uint64_t top[kMaxTop];                 // this CTA's k best
   uint64_t bars[kWarps * kStages];
   float m[kWarps], S[kWarps], A[kWarps];
   int before[kWarps], nan[kWarps];
-  unsigned short open[kThreads];         // threads whose elements are read again
+  unsigned char open[kThreads];          // threads whose elements are read again
   uint64_t tau;
   int n_open, n_list;
   float cm, cS, cA;                      // this CTA's sums
@@ -361,18 +364,6 @@ __global__ void __launch_bounds__(kThreads, kResident)
   }
   __syncwarp();
   pdl_wait_trigger();
-  const long long tok = tokens ? tokens[row] : -1;
-  const bool has_t = tok >= 0 && tok < V;
-  const int t = has_t ? (int)tok : -1;
-  const float xt = has_t ? Vec<X>::one(r.x + t) : INFINITY;
-  // what precedes the token: values above xt, and with a lower id those equal to
-  // it, i.e. above the next lower value
-  const uint32_t tb = has_t ? Vec<X>::bits(r.x + t) : 0u;
-  const uint32_t above_t = tb * Vec<X>::kPair;
-  const uint32_t from_t = ((tb & ~Vec<X>::kSign) == 0 ? Vec<X>::kSign | 1u : tb & Vec<X>::kSign ? tb + 1 : tb - 1) *
-                          Vec<X>::kPair;
-  const bool plain_t = fabsf(xt) < INFINITY;
-
   // ---- one pass: chunks of the row, dealt to the warps of the cluster in turn
   constexpr bool kFused = std::is_same<X, __half>::value;    // t in one multiply-add
   const F2 l2e(kLog2e, kLog2e);
@@ -388,6 +379,18 @@ __global__ void __launch_bounds__(kThreads, kResident)
     for (int j = 0; j < kStages; ++j)
       if (begin + j * stride < r.words && r.bulk(begin + j * stride))
         copy_chunk(ring + j * kChunk, r.at(begin + j * stride), &bars[j]);
+  const long long tok = tokens ? tokens[row] : -1;
+  const bool has_t = tok >= 0 && tok < V;
+  const int t = has_t ? (int)tok : -1;
+  const float xt = has_t ? Vec<X>::one(r.x + t) : INFINITY;
+  // what precedes the token: values above xt, and with a lower id those equal to
+  // it, i.e. above the next lower value
+  const uint32_t tb = has_t ? Vec<X>::bits(r.x + t) : 0u;
+  const uint32_t above_t = tb * Vec<X>::kPair;
+  const uint32_t from_t = ((tb & ~Vec<X>::kSign) == 0 ? Vec<X>::kSign | 1u : tb & Vec<X>::kSign ? tb + 1 : tb - 1) *
+                          Vec<X>::kPair;
+  const bool plain_t = fabsf(xt) < INFINITY;
+
   int stage = 0;
   unsigned parity = 0;                       // bit j: of stage j
   for (int base = begin; base < r.words; base += stride) {
@@ -571,39 +574,81 @@ __global__ void __launch_bounds__(kThreads, kResident)
     }
     __syncthreads();
     const uint64_t tau = sh.tau;
-    const bool again = upper >= tau && begin + lane < r.words;            // no bound: every thread's
+    const float tau_value = value_of(tau);
+    const bool again = upper >= tau && begin + lane < r.words;           // no bound: every thread's elements
     const unsigned who = __ballot_sync(0xffffffffu, again);
     int at = 0;
-    if (lane == 0 && who) at = atomicAdd(&sh.n_open, __popc(who));        // in any order, like the lists below:
-    at = __shfl_sync(0xffffffffu, at, 0);                                 // the keys are ranked in the end
-    if (again) sh.open[at + __popc(who & ((1u << lane) - 1))] = (unsigned short)tid;
+    if (lane == 0 && who) at = atomicAdd(&sh.n_open, __popc(who));       // in any order, like the list:
+    at = __shfl_sync(0xffffffffu, at, 0);                                // its keys are ranked in the end
+    if (again) sh.open[at + __popc(who & ((1u << lane) - 1))] = (unsigned char)tid;
     __syncthreads();
-    const int n_open = sh.n_open;
-    const float tau_value = value_of(tau);
-    uint64_t mine = 0;                                 // the warp's best so far, lane i the i-th
-    for (int q = warp; q < n_open; q += kWarps) {      // a thread's words, a chunk per four lanes
-      const int who = sh.open[q], first = (cta * kWarps + (who >> 5)) * kChunk + (who & 31);
-      for (int base = 0; first + base * stride < r.words; base += 32 / kUnroll) {
-        const int w = first + (base + lane / kUnroll) * stride + 32 * (lane % kUnroll);
-        const uint4 u = r.load(w);
-        if (tau && !__any_sync(0xffffffffu, !(Vec<X>::most(u) < tau_value))) continue;
-        float x[n];
-        Vec<X>::get(u, x);
+    const int per = ((r.words - cta * kWarps * kChunk + stride - 1) / stride) * kUnroll;   // words of a thread
+    const long work = (long)sh.n_open * per;
+    const bool few = tau && work <= 1 << 16;                             // exact in the division below
+    if (few) {
+      const float inv = 1.0f / (float)per;
+      constexpr int kAhead = 4;
+      for (int f = tid; f < (int)work; f += kAhead * kThreads) {
+        uint4 u[kAhead];
+        int w[kAhead];
 #pragma unroll
-        for (int j = 0; j < n; ++j) {
-          const int e = r.first(w) + j;
-          const uint64_t key = w < r.words && e >= 0 && e < V ? key_of(x[j], e) : 0ull;
-          const uint64_t floor = __shfl_sync(0xffffffffu, mine, k - 1);
-          unsigned in = __ballot_sync(0xffffffffu, key >= tau && key > floor);
-          for (; in; in &= in - 1) insert(mine, __shfl_sync(0xffffffffu, key, __ffs(in) - 1), lane);
+        for (int j = 0; j < kAhead; ++j) {
+          const int g = min(f + j * kThreads, (int)work - 1), q = (int)(((float)g + 0.5f) * inv), c = g - q * per;
+          const int o = sh.open[q];
+          w[j] = (cta * kWarps + (o >> 5)) * kChunk + (o & 31) + (c / kUnroll) * stride + 32 * (c % kUnroll);
+          if (f + j * kThreads >= (int)work) w[j] = r.words;
+          u[j] = r.load(w[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          if (Vec<X>::most(u[j]) < tau_value) continue;                  // NaN: goes on
+          float x[n];
+          Vec<X>::get(u[j], x);
+#pragma unroll
+          for (int i = 0; i < n; ++i)
+            if (x[i] >= tau_value && w[j] < r.words) {                   // finite: not what stands for outside the row
+              const uint64_t key = key_of(x[i], r.first(w[j]) + i);
+              if (key >= tau) {
+                const int to = atomicAdd(&sh.n_list, 1);
+                if (to < kList) sh.list[to] = key;
+              }
+            }
         }
       }
+      __syncthreads();
     }
-    const unsigned have = __ballot_sync(0xffffffffu, lane < k && mine);
-    if (lane == 0 && have) at = atomicAdd(&sh.n_list, __popc(have));
-    at = __shfl_sync(0xffffffffu, at, 0);
-    if (have >> lane & 1) sh.list[at + lane] = mine;
-    __syncthreads();
+    if (!few || sh.n_list > kList) {
+      __syncthreads();
+      if (tid == 0) sh.n_list = 0;
+      __syncthreads();
+      uint64_t mine = 0;                               // the warp's best so far, lane i the i-th
+      for (unsigned open = who; open; open &= open - 1) {   // a thread's words, a chunk per four lanes
+        const int first = begin + __ffs(open) - 1;
+        for (int base = 0; first + base * stride < r.words; base += 32 / kUnroll) {
+          const int w = first + (base + lane / kUnroll) * stride + 32 * (lane % kUnroll);
+          const uint4 u = r.load(w);
+          if (tau && !__any_sync(0xffffffffu, !(Vec<X>::most(u) < tau_value))) continue;
+          float x[n];
+          Vec<X>::get(u, x);
+#pragma unroll 1
+          for (int i = 0; i < n; ++i) {
+            const int e = r.first(w) + i;
+            float v = x[0];
+#pragma unroll
+            for (int q = 1; q < n; ++q) v = i == q ? x[q] : v;
+            const uint64_t key = w < r.words && e >= 0 && e < V ? key_of(v, e) : 0ull;
+            const uint64_t floor = __shfl_sync(0xffffffffu, mine, k - 1);
+            unsigned in = __ballot_sync(0xffffffffu, key >= tau && key > floor);
+            for (; in; in &= in - 1) insert(mine, __shfl_sync(0xffffffffu, key, __ffs(in) - 1), lane);
+          }
+        }
+      }
+      const unsigned have = __ballot_sync(0xffffffffu, lane < k && mine);
+      if (lane == 0 && have) at = atomicAdd(&sh.n_list, __popc(have));
+      at = __shfl_sync(0xffffffffu, at, 0);
+      if (have >> lane & 1) sh.list[at + lane] = mine;
+      __syncthreads();
+    }
     const int total = sh.n_list;
     for (int i = tid; i < total; i += kThreads) {
       const uint64_t key = sh.list[i];
