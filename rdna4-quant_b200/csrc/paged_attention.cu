@@ -45,6 +45,7 @@ namespace {
 __device__ int g_attn_status;
 
 constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
 constexpr int kSlots = 2;
 constexpr int kTile = 32;                         // positions per tile
 constexpr int kTileBytes = kTile * kHeadDim;      // of K, and of V
@@ -63,7 +64,7 @@ struct AttnArgs {
   __half* o;
   long ldo;
   int B, H, Hg, Hc, chunks, fwht;  // Hc: kv heads x groups of 8 query heads
-  FastDiv by_page, by_Hc, by_chunks;
+  FastDiv by_page, by_Hc, by_chunks, by_ctas;
   int per_seg;       // a CTA per (sequence, head, group) instead of equal runs
   int two_boxes;     // 16-position boxes
   int* header;       // workspace: tiles per CTA, then the prefix sums of tiles [B + 1]
@@ -146,13 +147,15 @@ struct Joined {
     }
   }
 };
-__device__ __forceinline__ void store_head(const AttnArgs& a, int b, int head, int kh, float L, float (&O)[4],
-                                           int lane) {
+__device__ __forceinline__ __half* out_head(const AttnArgs& a, int b, int head) {
+  return a.o + (long)b * a.ldo + (long)head * kHeadDim;
+}
+__device__ __forceinline__ void store_head(const AttnArgs& a, __half* o, int kh, float L, float (&O)[4], int lane) {
   const float inv = L > 0.f ? (a.c.v_scale ? a.c.v_scale[kh] : 1.f) / L : 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) O[i] *= inv;
   if (a.fwht) fwht32_x4(O, lane);
-  *reinterpret_cast<uint2*>(a.o + (long)b * a.ldo + (long)head * kHeadDim + 4 * lane) =
+  reinterpret_cast<uint2*>(o)[lane] =
       make_uint2(h2_as_u32(__floats2half2_rn(O[0], O[1])), h2_as_u32(__floats2half2_rn(O[2], O[3])));
 }
 
@@ -166,11 +169,14 @@ __device__ __forceinline__ Place place_of(const int* prefix, const AttnArgs& a, 
     const int mid = (lo + hi) >> 1;
     if (prefix[mid] <= y) lo = mid; else hi = mid;
   }
-  const int T = prefix[lo + 1] - prefix[lo], rem = x - prefix[lo] * a.Hc, hc = rem / T;
+  const int T = prefix[lo + 1] - prefix[lo], rem = x - prefix[lo] * a.Hc;
+  int hc = (int)__fdividef((float)rem, (float)T);     // below 2^16: off by one at most
+  hc -= hc * T > rem;
+  hc += (hc + 1) * T <= rem;
   return Place{lo, hc, rem - hc * T, T};
 }
 
-__global__ void __launch_bounds__(kWarps * 32, 1)
+__global__ void __launch_bounds__(kThreads, 1)
     paged_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                       const AttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
@@ -227,14 +233,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     __syncthreads();
   }
   const int N = prefix[a.B] * Hc;
-  // at least a tile per warp: fewer parts to join
-  const int per_cta = a.per_seg ? 0 : max(kWarps, (N + (int)gridDim.x - 1) / (int)gridDim.x);
+  // four tiles at least: fewer parts to join (8 against 4: 1 x 2048 8.0 against 7.0 us, 1 x 8192 11.8 against 11.2)
+  const int per_cta = a.per_seg ? 0 : max(4, a.by_ctas.div(N + (int)gridDim.x - 1));
   if (blockIdx.x == 0 && a.header)
-    for (int i = tid; i < a.B + 2; i += kWarps * 32) a.header[i] = i ? prefix[i - 1] : per_cta;
+    for (int i = tid; i < a.B + 2; i += kThreads) a.header[i] = i ? prefix[i - 1] : per_cta;
 
   for (int b = blockIdx.x; b < a.B; b += gridDim.x)
     if (prefix[b + 1] == prefix[b])                           // a sequence without a position
-      for (int i = tid; i < a.H * (kHeadDim / 8); i += kWarps * 32)
+      for (int i = tid; i < a.H * (kHeadDim / 8); i += kThreads)
         reinterpret_cast<uint4*>(a.o + (long)b * a.ldo)[i] = make_uint4(0, 0, 0, 0);
 
   // this CTA's run of the list, and this warp's
@@ -251,12 +257,15 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   const int beg = min(R1, R0 + warp * pw), end = min(R1, beg + pw);
 
   if (beg < end) {
-    Place at = place_of(prefix, a, beg);
+    Place at;
     int win = beg, pg0 = 0, pg1 = 0, row0 = 0, row1 = 0;      // coordinates of tile win + lane
     auto look_up = [&](int first) {
       win = first;
+      const Place p = place_of(prefix, a, min(first + lane, end - 1));
+      if (first == beg)                                       // where the warp begins
+        at = Place{__shfl_sync(0xffffffffu, p.b, 0), __shfl_sync(0xffffffffu, p.hc, 0),
+                   __shfl_sync(0xffffffffu, p.t, 0), __shfl_sync(0xffffffffu, p.T, 0)};
       if (first + lane < end) {
-        const Place p = place_of(prefix, a, first + lane);
         const int pos = p.t * kTile, kh = a.by_chunks.div(p.hc), blk = a.by_page.div(pos);
         const int* tab = a.c.table + (long)p.b * a.c.ld_table;
         pg0 = tab[blk];
@@ -288,6 +297,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
         }
       }
     };
+    look_up(beg);
     uint32_t qa[8], qb[8];
     float m = -1e30f, l = 0.f, scale = 0.f, oacc[16][4];
     int seq = 0;
@@ -311,12 +321,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
         for (int i = 0; i < 4; ++i) oacc[j][i] = 0.f;
     };
     start_segment();
-
-    look_up(beg);
 #pragma unroll
     for (int s = 0; s < kSlots; ++s)
       if (beg + s < end) issue(beg + s, s);
-
     int slot = 0;
     unsigned parity = 0;
     for (int x = beg; x < end; ++x) {
@@ -468,39 +475,24 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   }
   __syncthreads();
 
-  // ---- join the parts of this CTA, segment by segment; a warp per head
+  // ---- join the parts of this CTA, segment by segment; a warp per head.
   // Lane 2 w + which looks at part (w, which): it opens a segment of this CTA if it
   // is the head of the first warp, or a tail that does not go on from the warp
   // before; then come the tails of the next warps, up to the head that closes it.
-  unsigned open = 0;
-  int mine = -1, parts = 0;
-  if (lane < 2 * kWarps) {
-    const int w = lane >> 1;
-    mine = meta[lane];
-    if (mine >= 0 && (lane & 1 ? w == 0 || meta[lane - 2] != mine : w == 0)) {
-      parts = 1;
-      if (lane & 1)
-        for (int u = w + 1; u < kWarps; ++u) {
-          const int h = meta[2 * u];
-          if (h != mine && meta[2 * u + 1] != mine) break;
-          ++parts;
-          if (h == mine) break;
-        }
-    }
-  }
-  for (open = __ballot_sync(0xffffffffu, parts > 0); open; open &= open - 1) {
-    const int from = __ffs(open) - 1, w = from >> 1;
-    const int seg = __shfl_sync(0xffffffffu, mine, from), n = __shfl_sync(0xffffffffu, parts, from);
+  const int mine = lane < 2 * kWarps ? meta[lane] : -1, before = __shfl_up_sync(0xffffffffu, mine, 2);
+  const bool opens = mine >= 0 && ((lane & 1) ? lane < 2 || before != mine : lane == 0);
+  for (unsigned open = __ballot_sync(0xffffffffu, opens); open; open &= open - 1) {
+    const int from = __ffs(open) - 1, seg = __shfl_sync(0xffffffffu, mine, from), w = from >> 1;
+    const unsigned of = __ballot_sync(0xffffffffu, mine == seg), heads = of & 0x55555555u;
     const int b = a.by_Hc.div(seg), hc = seg - b * Hc, T = prefix[b + 1] - prefix[b], s0 = prefix[b] * Hc + hc * T;
     const int kh = a.by_chunks.div(hc), hg = (hc - kh * a.chunks) * kGroup + warp;
     if (hg >= a.Hg) continue;
     Joined j;
-    j.add_all(0, 1, n, lane, [&](int i) {
-      const int u = w + i;
-      return part0 + (2 * u + (meta[2 * u] == seg ? 0 : 1)) * kPartFloats + warp * kPitch;
+    j.add_all(0, 1, __popc(of), lane, [&](int i) {
+      return part0 + (2 * (w + i) + (heads >> (2 * (w + i)) & 1 ? 0 : 1)) * kPartFloats + warp * kPitch;
     });
     if (s0 >= R0 && s0 + T <= R1)
-      store_head(a, b, kh * a.Hg + hg, kh, j.L, j.O, lane);
+      store_head(a, out_head(a, b, kh * a.Hg + hg), kh, j.L, j.O, lane);
     else
       j.put(a.parts + ((long)blockIdx.x * 2 + (s0 < R0 ? 0 : 1)) * kPartFloats + warp * kPitch, lane);
   }
@@ -510,10 +502,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
 // head, its warps take every fourth part.
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const AttnArgs a) {
   __shared__ float part[kJoinWarps][kPitch];
-  pdl_wait_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = blockIdx.x, b = blockIdx.y, kh = head / a.Hg, hg = head - kh * a.Hg;
   const int hc = kh * a.chunks + hg / kGroup;
+  pdl_wait_trigger();
   const int per_cta = a.header[0], p0 = a.header[1 + b], T = a.header[2 + b] - p0;
   const int s0 = p0 * a.Hc + hc * T, c0 = s0 / per_cta, c1 = (s0 + T - 1) / per_cta;
   if (T == 0 || c0 == c1) return;
@@ -526,7 +518,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const AttnA
   if (warp) return;
   Joined all;
   all.add_all(0, 1, kJoinWarps, lane, [&](int i) { return part[i]; });
-  store_head(a, b, head, kh, all.L, all.O, lane);
+  store_head(a, out_head(a, b, head), kh, all.L, all.O, lane);
 }
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -611,13 +603,14 @@ extern "C" int r4q_paged_flash_decode(const void* q, long ldq, const r4q_paged_c
   a.chunks = (a.Hg + kGroup - 1) / kGroup;
   const int Hc = a.Hc = groups_of(H, a.c.Hk);
   const long cap = (long)a.c.max_blocks * a.c.page;
-  if ((cap / kTile + 1) * B * Hc > 0x7fffffffL - 65536)
+  if ((cap / kTile + 1) * B * Hc > 1L << 30)
     return set_error(R4Q_ERR_ARG, "paged_flash_decode: %d sequences of %ld positions and %d heads are too many tiles",
                      B, cap, Hc);
   a.per_seg = per_segment(B * Hc, a.c.page, a.c.max_blocks);
   a.by_page = fast_div(a.c.page);
   a.by_Hc = fast_div(Hc);
   a.by_chunks = fast_div(a.chunks);
+  a.by_ctas = fast_div(num_sms());
   const size_t need = a.per_seg ? 0 : r4q_paged_flash_decode_workspace_bytes(B, H, a.c.Hk, a.c.page, a.c.max_blocks);
   if (need && (!workspace || ws_bytes < need))
     return set_error(R4Q_ERR_CAPACITY, "paged_flash_decode: workspace %zu < %zu bytes", ws_bytes, need);
@@ -654,7 +647,7 @@ extern "C" int r4q_paged_flash_decode(const void* q, long ldq, const r4q_paged_c
   }
   cudaStream_t s = (cudaStream_t)stream;
   const unsigned ctas = a.per_seg ? (unsigned)(B * Hc) : (unsigned)num_sms();
-  cudaError_t e = launch_pdl(paged_attn_kernel, dim3(ctas), dim3(kWarps * 32), smem_bytes(B), s, tmk, tmv, a);
+  cudaError_t e = launch_pdl(paged_attn_kernel, dim3(ctas), dim3(kThreads), smem_bytes(B), s, tmk, tmv, a);
   if (e == cudaSuccess && !a.per_seg)
     e = launch_pdl(paged_join_kernel, dim3((unsigned)H, (unsigned)B), dim3(kJoinWarps * 32), 0, s, a);
   if (e != cudaSuccess) {
