@@ -435,28 +435,33 @@ def _run_on(index: int, name: str, *args) -> None:
 
 
 def _heads(t: torch.Tensor, name: str, rows: Optional[int] = None, heads: Optional[int] = None, out: bool = False):
-    """(t, row stride) of fp16 [rows, heads, 128] with the heads of a row side
-    by side; an input laid out otherwise is copied, an output refused."""
+    """(t, rows, heads, row stride) of fp16 [rows, heads, 128] with the heads of
+    a row side by side; an input laid out otherwise is copied, an output refused."""
     if t.dtype is not torch.float16:
         raise TypeError(f"{name} must be float16")
     sh = t.shape
     if len(sh) != 3 or sh[2] != 128 or (rows is not None and sh[0] != rows) or (heads is not None and sh[1] != heads):
-        raise ValueError(f"{name} must be [{rows or 'rows'}, {heads or 'heads'}, 128], got {tuple(sh)}")
-    width = sh[1] * 128
-    st = t.stride()
-    if st == (width, 128, 1):
-        return t, width
-    if t.numel() and (st[2] != 1 or (sh[1] > 1 and st[1] != 128) or (sh[0] > 1 and st[0] < width)):
-        if out:
-            raise ValueError(f"{name} must hold the heads of a row side by side")
-        return t.contiguous(), width
-    return t, st[0] if sh[0] > 1 else width
+        raise ValueError(f"{name} must be [{'rows' if rows is None else rows}, {'heads' if heads is None else heads}, "
+                         f"128], got {tuple(sh)}")
+    r, h, _ = sh
+    ld, st, one = t.stride()
+    if one != 1 or st != 128 or ld < h * 128:        # a dimension of one element may have any stride
+        if (one != 1 or (st != 128 and h > 1) or (ld < h * 128 and r > 1)) and r and h:
+            if out:
+                raise ValueError(f"{name} must hold the heads of a row side by side")
+            t = t.contiguous()
+        ld = t.stride(0) if r > 1 else h * 128
+    return t, r, h, ld
 
 
 def _vector(t: torch.Tensor, name: str, dtype: torch.dtype, n: int) -> torch.Tensor:
-    if t.dtype is not dtype or t.shape != (n,):
+    if t.dtype is not dtype or t.dim() != 1 or t.numel() != n:
         raise ValueError(f"{name} must be {str(dtype)[6:]} [{n}], got {str(t.dtype)[6:]} {tuple(t.shape)}")
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _contiguous_vector(t: torch.Tensor, dtype: torch.dtype, n: int) -> bool:
+    return t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous()
 
 
 def _paged_cache(k_pages, v_pages, block_table, k_scale, v_scale):
@@ -468,23 +473,26 @@ def _paged_cache(k_pages, v_pages, block_table, k_scale, v_scale):
         raise ValueError("k_pages and v_pages must be [pages, kv heads, page, 128] of one shape, got "
                          f"{tuple(sh)} and {tuple(v_pages.shape)}")
     P, Hk, page, _ = sh
-    ks, vs, inner = k_pages.stride(), v_pages.stride(), (page * 128, 128, 1)
-    for st in (ks, vs):
-        if st[1:] != inner and (st[2:] != inner[1:] or Hk > 1):
-            raise ValueError("each page must be contiguous [kv heads, page, 128]")
+    k_stride, *k_inner = k_pages.stride()
+    v_stride, *v_inner = v_pages.stride()
+    inner = [page * 128, 128, 1]
+    if (k_inner != inner or v_inner != inner) and (Hk > 1 or k_inner[1:] != inner[1:] or v_inner[1:] != inner[1:]):
+        raise ValueError("each page must be contiguous [kv heads, page, 128]")
     if block_table.dtype is not torch.int32 or block_table.dim() != 2:
         raise TypeError("block_table must be int32 [sequences, blocks]")
     S, nb = block_table.shape
     ld, one = block_table.stride()
     if one != 1 and nb > 1:
         raise ValueError("block_table rows must be contiguous")
-    for s in (k_scale, v_scale):
-        if s is not None and (s.dtype is not torch.float32 or s.shape != (Hk,) or not s.is_contiguous()):
-            raise ValueError(f"k_scale and v_scale must be float32 [{Hk}], one per kv head")
-    return L.PAGED_CACHE.pack(k_pages.data_ptr(), v_pages.data_ptr(), ks[0] if P > 1 else 0, vs[0] if P > 1 else 0, P,
-                              page, Hk, block_table.data_ptr(), ld if S > 1 else nb, S, nb,
-                              0 if k_scale is None else k_scale.data_ptr(),
-                              0 if v_scale is None else v_scale.data_ptr()), Hk, page, nb
+    ks = vs = 0
+    if k_scale is not None or v_scale is not None:
+        for s in (k_scale, v_scale):
+            if s is not None and not _contiguous_vector(s, torch.float32, Hk):
+                raise ValueError(f"k_scale and v_scale must be float32 [{Hk}], one per kv head")
+        ks, vs = _ptr(k_scale) or 0, _ptr(v_scale) or 0
+    return L.PAGED_CACHE.pack(k_pages.data_ptr(), v_pages.data_ptr(), k_stride if P > 1 else 0,
+                              v_stride if P > 1 else 0, P, page, Hk, block_table.data_ptr(), ld if S > 1 else nb, S,
+                              nb, ks, vs), Hk, page, nb
 
 
 def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -507,40 +515,40 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     gpu = _same_gpu(k, v, k_pages, v_pages, block_table, positions, rows, q, q_w, k_w, cos, sin, q_out, k_out, k_scale,
                     v_scale)
     cache, Hk, _, _ = _paged_cache(k_pages, v_pages, block_table, k_scale, v_scale)
-    k, ldk = _heads(k, "k", heads=Hk)
-    M = k.shape[0]
-    v, ldv = _heads(v, "v", M, Hk)
+    k, M, _, ldk = _heads(k, "k", None, Hk)
+    v, _, _, ldv = _heads(v, "v", M, Hk)
     positions = _vector(positions, "positions", torch.int64, M)
     if rows is not None:
         rows = _vector(rows, "rows", torch.int32, M)
     H = ldq = ldqo = ldko = tab_stride = tab_rows = 0
     flags = L.KV_FULL_RANGE if full_range else 0
     if q is not None:
-        q, ldq = _heads(q, "q", M)
-        H = q.shape[1]
+        q, _, H, ldq = _heads(q, "q", M)
         if q_out is None:
             q_out, ldqo = torch.empty(M, H, 128, dtype=torch.float16, device=q.device), H * 128
         else:
-            q_out, ldqo = _heads(q_out, "q_out", M, H, out=True)
+            q_out, _, _, ldqo = _heads(q_out, "q_out", M, H, True)
     elif q_out is not None or q_w is not None:
         raise ValueError("q_out and q_w need q")
     if k_out is not None:
-        k_out, ldko = _heads(k_out, "k_out", M, Hk, out=True)
+        k_out, _, _, ldko = _heads(k_out, "k_out", M, Hk, True)
     if k_w is not None or q_w is not None:
         if k_w is None or (q is not None and q_w is None):
             raise ValueError("the norm needs a weight for q and for k")
-        for w in (q_w, k_w):
-            if w is not None and (w.dtype is not torch.float16 or w.shape != (128,) or not w.is_contiguous()):
-                raise ValueError("norm weights must be float16 [128]")
+        if not _contiguous_vector(k_w, torch.float16, 128) or \
+                (q_w is not None and not _contiguous_vector(q_w, torch.float16, 128)):
+            raise ValueError("norm weights must be float16 [128]")
         flags |= L.HEAD_NORM
     if cos is not None or sin is not None:
         if cos is None or sin is None or cos.dtype is not torch.float16 or sin.dtype is not torch.float16 or \
-                cos.dim() != 2 or cos.shape[1] < 64 or sin.shape != cos.shape or cos.stride(1) != 1 or \
-                sin.stride() != cos.stride():
+                cos.dim() != 2 or sin.shape != cos.shape or sin.stride() != cos.stride():
             raise ValueError("cos and sin must be float16 [rows, 64] of one layout")
+        tab_rows, half = cos.shape
+        tab_stride, one = cos.stride()
+        if half < 64 or one != 1:
+            raise ValueError("cos and sin must be float16 [rows, 64] with contiguous rows")
+        tab_stride = tab_stride if tab_rows > 1 else 64
         flags |= L.HEAD_ROPE
-        tab_rows = cos.shape[0]
-        tab_stride = cos.stride(0) if tab_rows > 1 else 64
     _run_on(gpu, "r4q_paged_kv_write", _ptr(q), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, _ptr(q_w), _ptr(k_w),
             _ptr(cos), _ptr(sin), tab_stride, tab_rows, _ptr(q_out), ldqo, _ptr(k_out), ldko, cache, _ptr(rows),
             positions.data_ptr(), M, H, eps, flags)
@@ -565,14 +573,13 @@ def paged_flash_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     torch's allocator at every call, so calls on several streams and captured
     graphs share nothing."""
     gpu = _same_gpu(q, k_pages, v_pages, block_table, seq_lens, k_scale, v_scale, out)
-    q, ldq = _heads(q, "q")
-    B, H, _ = q.shape
+    q, B, H, ldq = _heads(q, "q")
     cache, Hk, page, nb = _paged_cache(k_pages, v_pages, block_table, k_scale, v_scale)
     seq_lens = _vector(seq_lens, "seq_lens", torch.int64, B)
     if out is None:
         out, ldo = torch.empty(B, H, 128, dtype=torch.float16, device=q.device), H * 128
     else:
-        out, ldo = _heads(out, "out", B, H, out=True)
+        out, _, _, ldo = _heads(out, "out", B, H, True)
     need = _paged_workspace_bytes(gpu, B, H, Hk, page, nb)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     _run_on(gpu, "r4q_paged_flash_decode", q.data_ptr(), ldq, cache, seq_lens.data_ptr(), out.data_ptr(), ldo, B, H,
