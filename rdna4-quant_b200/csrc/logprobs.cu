@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, kResident)
   unsigned parity = 0;                       // bit j: of stage j
   for (int base = begin; base < r.words; base += stride) {
     const int i = base + lane;               // this lane's words: i, i + 32, ..
-    uint4 u[kUnroll];
+    uint4* mine = ring + stage * kChunk + lane;
     if (r.bulk(base)) {
       if (!wait_full(&bars[stage], parity >> stage & 1)) {
         // the copies in flight get their time once more; the row's results are void
@@ -408,29 +408,27 @@ __global__ void __launch_bounds__(kThreads, kResident)
         break;
       }
       parity ^= 1u << stage;
-#pragma unroll
-      for (int j = 0; j < kUnroll; ++j) u[j] = ring[stage * kChunk + lane + 32 * j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < kUnroll; ++j) u[j] = r.load(i + 32 * j);
+    } else {                                 // a chunk at the row's ends: every lane puts its own words there
+#pragma unroll 1
+      for (int j = 0; j < kUnroll; ++j) mine[32 * j] = r.load(i + 32 * j);
     }
-    __syncwarp();
-    if (lane == 0) {                         // the stage is in registers: its next chunk may come
-      const int at = base + kStages * stride;
-      if (at < r.words && r.bulk(at)) {
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        copy_chunk(ring + stage * kChunk, r.at(at), &bars[stage]);
-      }
+    // words are read from shared memory again where they are used: held in registers
+    // throughout, they and what is made of them exceed the 64 of four CTAs an SM
+    const uint32_t words = smem_u32(mine);
+    float c;
+    {
+      uint4 u[kUnroll];
+#pragma unroll
+      for (int j = 0; j < kUnroll; ++j) u[j] = lds128(words + 512 * j);
+      c = Vec<X>::most4(u);
     }
-    stage = stage + 1 == kStages ? 0 : stage + 1;
-    float c = Vec<X>::most4(u);
     if (c != c) {                            // NaN: the row is none; the order goes on without it
       nan = 1;
       c = -INFINITY;
-#pragma unroll
+#pragma unroll 1
       for (int j = 0; j < kUnroll; ++j) {
         float x[n];
-        Vec<X>::get(u[j], x);
+        Vec<X>::get(lds128(words + 512 * j), x);
 #pragma unroll
         for (int q = 0; q < n; ++q) c = fmaxf(c, x[q]);
       }
@@ -448,23 +446,39 @@ __global__ void __launch_bounds__(kThreads, kResident)
       M = to;
       shift = F2(-to, -to);
     }
-    const bool count = has_t && (c >= xt || xt != xt);
+    // the chunk's sums; -inf gives 0 * -inf in A, and only then t is bounded below
+    F2 Ac(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
       float x[n];
-      Vec<X>::get(u[j], x);
+      Vec<X>::get(lds128(words + 512 * j), x);
 #pragma unroll
       for (int q = 0; q < n; q += 2) {
-        const F2 two(x[q], x[q + 1]);
-        float2 t2 = (kFused ? fma(two, l2e, shift) : mul(add(two, shift), l2e)).get();
-        t2.x = fmaxf(t2.x, kTiny);
-        t2.y = fmaxf(t2.y, kTiny);
-        const F2 e(ex2(t2.x), ex2(t2.y));
+        const F2 two(x[q], x[q + 1]), t = kFused ? fma(two, l2e, shift) : mul(add(two, shift), l2e);
+        const float2 f = t.get();
+        const F2 e(ex2(f.x), ex2(f.y));
         S2 = add(S2, e);
-        A2 = fma(e, F2(t2.x, t2.y), A2);
+        Ac = fma(e, t, Ac);
       }
     }
-    if (count) {
+    const float2 sum = Ac.get();
+    if (sum.x + sum.y != sum.x + sum.y) {
+      Ac = F2(0.f, 0.f);
+#pragma unroll 1
+      for (int j = 0; j < kUnroll; ++j) {
+        float x[n];
+        Vec<X>::get(lds128(words + 512 * j), x);
+#pragma unroll
+        for (int q = 0; q < n; q += 2) {
+          const F2 two(x[q], x[q + 1]);
+          const float2 f = (kFused ? fma(two, l2e, shift) : mul(add(two, shift), l2e)).get();
+          const F2 t(fmaxf(f.x, kTiny), fmaxf(f.y, kTiny));
+          Ac = fma(F2(ex2(fmaxf(f.x, kTiny)), ex2(fmaxf(f.y, kTiny))), t, Ac);
+        }
+      }
+    }
+    A2 = add(A2, Ac);
+    if (has_t && (c >= xt || xt != xt)) {    // what precedes the token
       uint32_t th[kUnroll];
       bool has = !plain_t;
 #pragma unroll
@@ -474,13 +488,16 @@ __global__ void __launch_bounds__(kThreads, kResident)
         has |= (unsigned)(t - e0) < (unsigned)n;
       }
       if (!has) {
+        uint4 u[kUnroll];
+#pragma unroll
+        for (int j = 0; j < kUnroll; ++j) u[j] = lds128(words + 512 * j);
         before += Vec<X>::above(u, th);
       } else {                               // the token's own chunk; a token of no finite value
-#pragma unroll
+#pragma unroll 1
         for (int j = 0; j < kUnroll; ++j) {
           const int e0 = r.first(i + 32 * j);
           float x[n];
-          Vec<X>::get(u[j], x);
+          Vec<X>::get(lds128(words + 512 * j), x);
 #pragma unroll
           for (int q = 0; q < n; ++q) {
             const unsigned e = (unsigned)(e0 + q);
@@ -490,6 +507,15 @@ __global__ void __launch_bounds__(kThreads, kResident)
         }
       }
     }
+    __syncwarp();
+    if (lane == 0) {                         // the stage is read: its next chunk may come
+      const int at = base + kStages * stride;
+      if (at < r.words && r.bulk(at)) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        copy_chunk(ring + stage * kChunk, r.at(at), &bars[stage]);
+      }
+    }
+    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
   Sums s;
   s.m = most;
