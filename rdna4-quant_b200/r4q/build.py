@@ -1,4 +1,5 @@
-"""Build ``libr4q.so`` (all of csrc/*.cu) in-tree with nvcc for sm_100a.
+"""Build ``libr4q.so`` (all of csrc/*.cu) in-tree with nvcc for sm_100a, and the
+Python module ``_r4q_torch`` (csrc/torch_ops.cpp) against the installed torch.
 
     python -m r4q.build        (from the rdna4-quant_b200 folder)
 
@@ -10,12 +11,15 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent.parent
 CSRC = PKG / "csrc"
 OUT = PKG / "libr4q.so"
+TORCH_SRC = CSRC / "torch_ops.cpp"
+TORCH_OUT = PKG / "_r4q_torch.so"
 BUILD = PKG / "_build"
 INCLUDE = PKG.parent / "include"
 
@@ -42,6 +46,18 @@ def _stale(obj: Path, src: Path, headers) -> bool:
     return src.stat().st_mtime > t or any(h.stat().st_mtime > t for h in headers)
 
 
+def _torch_command(out: Path) -> list:
+    """nvcc passes a .cpp file on to its host compiler, the one of the .cu files: one C++ runtime, the shared one
+    that torch uses (a compiler that links its own copy statically breaks streams and exceptions across the two)."""
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    return [_nvcc(), "-O2", "-std=c++17", "-shared", "--cudart=none", "-Xcompiler", "-fPIC",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{root / 'include'}",
+            f"-I{root / 'include/torch/csrc/api/include'}", f"-I{sysconfig.get_paths()['include']}", str(TORCH_SRC),
+            "-o", str(out), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+            "-Xlinker", f"-rpath,{root / 'lib'}"]
+
+
 def build(verbose: bool = False, force: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     headers = list(CSRC.glob("*.cuh")) + list(INCLUDE.glob("*.h"))
@@ -62,8 +78,15 @@ def build(verbose: bool = False, force: bool = False) -> Path:
             raise RuntimeError(f"nvcc failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
         return r
 
+    module = TORCH_OUT.with_suffix(".so.tmp")
+    stale_module = force or _stale(TORCH_OUT, TORCH_SRC, [INCLUDE / "r4q.h"])
+    if stale_module:
+        jobs.insert(0, _torch_command(module))      # the longest first
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
         list(ex.map(run, jobs))
+    if stale_module:
+        os.replace(module, TORCH_OUT)
+        jobs.pop(0)
     if jobs or force or not OUT.exists() or any(o.stat().st_mtime > OUT.stat().st_mtime for o in objs):
         tmp = OUT.with_suffix(".so.tmp")
         run([nvcc, *ARCH, "-shared", "-o", str(tmp), *map(str, objs), "-lcudart"])

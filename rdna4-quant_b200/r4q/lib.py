@@ -65,8 +65,7 @@ class ModelDesc(C.Structure):
 
 
 # r4q_paged_cache (include/r4q.h) in the platform's C layout: k_pages, v_pages, k_stride, v_stride, n_pages, page, Hk,
-# table, ld_table, seqs, max_blocks, k_scale, v_scale (0: NULL).  The packed bytes are passed as the pointer, which
-# costs a fraction of building a ctypes.Structure per call.
+# table, ld_table, seqs, max_blocks, k_scale, v_scale (0: NULL); the packed bytes are passed as the pointer
 PAGED_CACHE = struct.Struct("@PPlliiiPliiPP")
 
 _SIGS = {

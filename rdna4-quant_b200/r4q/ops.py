@@ -3,10 +3,9 @@ per-(device, stream) GEMV workspaces.  Device memory and streams come from
 PyTorch; all arithmetic runs in libr4q.so."""
 from __future__ import annotations
 
-import array
 import ctypes as C
+import importlib.util
 import threading
-from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
@@ -20,13 +19,10 @@ _ws: dict = {}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def stream_handle(dev) -> int:
-    """cudaStream_t of torch's current stream on dev, a torch.device or an
-    index (the raw-handle query costs a fraction of building a
-    torch.cuda.Stream object per call)."""
+def stream_handle(dev: torch.device) -> int:
+    """cudaStream_t of torch's current stream on dev (the raw-handle query
+    costs a fraction of building a torch.cuda.Stream object per call)."""
     if _raw_stream is not None:
-        if isinstance(dev, int):
-            return _raw_stream(dev)
         return _raw_stream(dev.index if dev.index is not None else torch.cuda.current_device())
     return torch.cuda.current_stream(dev).cuda_stream
 
@@ -414,85 +410,30 @@ def residual_f16(a: torch.Tensor, res: torch.Tensor | None, out: torch.Tensor, s
 
 
 # ------------------------------------------------------------- paged KV cache ---
-def _same_gpu(t: torch.Tensor, *others) -> int:
-    """Index of the one GPU that holds every tensor (None: not given)."""
-    i = t.get_device()
-    for o in others:
-        if o is not None and o.get_device() != i:
-            raise ValueError("all tensors must be on the same CUDA device")
-    if i < 0:
-        raise ValueError("r4q ops take CUDA tensors only (no CPU fallback)")
-    return i
+# The operators from here on check their tensors and allocate in the native
+# module _r4q_torch (csrc/torch_ops.cpp), which calls the library that lib.py loaded.
+def _load_native():
+    path = L._PKG / "_r4q_torch.so"
+    if not path.exists():
+        raise ImportError(f"_r4q_torch.so not found at {path}: build it with `python -m r4q.build` "
+                          "(or __graft_entry__.build()); r4q has no CPU fallback")
+    spec = importlib.util.spec_from_file_location("_r4q_torch", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    mod.bind(*(C.cast(getattr(L.LIB, n), C.c_void_p).value for n in (
+        "r4q_paged_kv_write", "r4q_paged_flash_decode", "r4q_paged_flash_decode_workspace_bytes",
+        "r4q_kv_copy_pages", "r4q_kv_table_set", "r4q_token_logprobs")))
+    return mod
 
 
-def _run_on(index: int, name: str, *args) -> None:
-    """L.call with the GPU's current stream as the last argument and that GPU current."""
-    if index == torch.cuda.current_device():
-        L.call(name, *args, stream_handle(index))
-    else:
-        with torch.cuda.device(index):
-            L.call(name, *args, stream_handle(index))
+_native = _load_native()
 
 
-def _heads(t: torch.Tensor, name: str, rows: Optional[int] = None, heads: Optional[int] = None, out: bool = False):
-    """(t, rows, heads, row stride) of fp16 [rows, heads, 128] with the heads of
-    a row side by side; an input laid out otherwise is copied, an output refused."""
-    if t.dtype is not torch.float16:
-        raise TypeError(f"{name} must be float16")
-    sh = t.shape
-    if len(sh) != 3 or sh[2] != 128 or (rows is not None and sh[0] != rows) or (heads is not None and sh[1] != heads):
-        raise ValueError(f"{name} must be [{'rows' if rows is None else rows}, {'heads' if heads is None else heads}, "
-                         f"128], got {tuple(sh)}")
-    r, h, _ = sh
-    ld, st, one = t.stride()
-    if one != 1 or st != 128 or ld < h * 128:        # a dimension of one element may have any stride
-        if (one != 1 or (st != 128 and h > 1) or (ld < h * 128 and r > 1)) and r and h:
-            if out:
-                raise ValueError(f"{name} must hold the heads of a row side by side")
-            t = t.contiguous()
-        ld = t.stride(0) if r > 1 else h * 128
-    return t, r, h, ld
-
-
-def _vector(t: torch.Tensor, name: str, dtype: torch.dtype, n: int) -> torch.Tensor:
-    if t.dtype is not dtype or t.dim() != 1 or t.numel() != n:
-        raise ValueError(f"{name} must be {str(dtype)[6:]} [{n}], got {str(t.dtype)[6:]} {tuple(t.shape)}")
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _contiguous_vector(t: torch.Tensor, dtype: torch.dtype, n: int) -> bool:
-    return t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous()
-
-
-def _paged_cache(k_pages, v_pages, block_table, k_scale, v_scale):
-    """(packed r4q_paged_cache, Hk, page, max_blocks) of checked tensors."""
-    if k_pages.dtype is not torch.uint8 or v_pages.dtype is not torch.uint8:
-        raise TypeError("pages must be uint8 (FP8 E4M3 bytes)")
-    sh = k_pages.shape
-    if len(sh) != 4 or sh[3] != 128 or v_pages.shape != sh:
-        raise ValueError("k_pages and v_pages must be [pages, kv heads, page, 128] of one shape, got "
-                         f"{tuple(sh)} and {tuple(v_pages.shape)}")
-    P, Hk, page, _ = sh
-    k_stride, *k_inner = k_pages.stride()
-    v_stride, *v_inner = v_pages.stride()
-    inner = [page * 128, 128, 1]
-    if (k_inner != inner or v_inner != inner) and (Hk > 1 or k_inner[1:] != inner[1:] or v_inner[1:] != inner[1:]):
-        raise ValueError("each page must be contiguous [kv heads, page, 128]")
-    if block_table.dtype is not torch.int32 or block_table.dim() != 2:
-        raise TypeError("block_table must be int32 [sequences, blocks]")
-    S, nb = block_table.shape
-    ld, one = block_table.stride()
-    if one != 1 and nb > 1:
-        raise ValueError("block_table rows must be contiguous")
-    ks = vs = 0
-    if k_scale is not None or v_scale is not None:
-        for s in (k_scale, v_scale):
-            if s is not None and not _contiguous_vector(s, torch.float32, Hk):
-                raise ValueError(f"k_scale and v_scale must be float32 [{Hk}], one per kv head")
-        ks, vs = _ptr(k_scale) or 0, _ptr(v_scale) or 0
-    return L.PAGED_CACHE.pack(k_pages.data_ptr(), v_pages.data_ptr(), k_stride if P > 1 else 0,
-                              v_stride if P > 1 else 0, P, page, Hk, block_table.data_ptr(), ld if S > 1 else nb, S,
-                              nb, ks, vs), Hk, page, nb
+def _checked(r, name: str):
+    """A native result; a status from the C entry point becomes R4QError."""
+    if type(r) is int:
+        raise L.R4QError(r, name, L.last_error())
+    return r
 
 
 def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -512,53 +453,9 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     enc(x / scale), the bytes of the contiguous cache; ``full_range`` keeps
     256 .. 448 apart, which its codec stores as 448.  Rows, positions and page
     ids out of range write nothing and are reported by ``check_status``."""
-    gpu = _same_gpu(k, v, k_pages, v_pages, block_table, positions, rows, q, q_w, k_w, cos, sin, q_out, k_out, k_scale,
-                    v_scale)
-    cache, Hk, _, _ = _paged_cache(k_pages, v_pages, block_table, k_scale, v_scale)
-    k, M, _, ldk = _heads(k, "k", None, Hk)
-    v, _, _, ldv = _heads(v, "v", M, Hk)
-    positions = _vector(positions, "positions", torch.int64, M)
-    if rows is not None:
-        rows = _vector(rows, "rows", torch.int32, M)
-    H = ldq = ldqo = ldko = tab_stride = tab_rows = 0
-    flags = L.KV_FULL_RANGE if full_range else 0
-    if q is not None:
-        q, _, H, ldq = _heads(q, "q", M)
-        if q_out is None:
-            q_out, ldqo = torch.empty(M, H, 128, dtype=torch.float16, device=q.device), H * 128
-        else:
-            q_out, _, _, ldqo = _heads(q_out, "q_out", M, H, True)
-    elif q_out is not None or q_w is not None:
-        raise ValueError("q_out and q_w need q")
-    if k_out is not None:
-        k_out, _, _, ldko = _heads(k_out, "k_out", M, Hk, True)
-    if k_w is not None or q_w is not None:
-        if k_w is None or (q is not None and q_w is None):
-            raise ValueError("the norm needs a weight for q and for k")
-        if not _contiguous_vector(k_w, torch.float16, 128) or \
-                (q_w is not None and not _contiguous_vector(q_w, torch.float16, 128)):
-            raise ValueError("norm weights must be float16 [128]")
-        flags |= L.HEAD_NORM
-    if cos is not None or sin is not None:
-        if cos is None or sin is None or cos.dtype is not torch.float16 or sin.dtype is not torch.float16 or \
-                cos.dim() != 2 or sin.shape != cos.shape or sin.stride() != cos.stride():
-            raise ValueError("cos and sin must be float16 [rows, 64] of one layout")
-        tab_rows, half = cos.shape
-        tab_stride, one = cos.stride()
-        if half < 64 or one != 1:
-            raise ValueError("cos and sin must be float16 [rows, 64] with contiguous rows")
-        tab_stride = tab_stride if tab_rows > 1 else 64
-        flags |= L.HEAD_ROPE
-    _run_on(gpu, "r4q_paged_kv_write", _ptr(q), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, _ptr(q_w), _ptr(k_w),
-            _ptr(cos), _ptr(sin), tab_stride, tab_rows, _ptr(q_out), ldqo, _ptr(k_out), ldko, cache, _ptr(rows),
-            positions.data_ptr(), M, H, eps, flags)
-    return q_out
-
-
-@lru_cache(maxsize=256)
-def _paged_workspace_bytes(gpu: int, B: int, H: int, Hk: int, page: int, max_blocks: int) -> int:
-    with torch.cuda.device(gpu):
-        return L.LIB.r4q_paged_flash_decode_workspace_bytes(B, H, Hk, page, max_blocks)
+    return _checked(_native.paged_kv_write(k, v, k_pages, v_pages, block_table, positions, rows, q, q_w, k_w, cos, sin,
+                                           q_out, k_out, k_scale, v_scale, eps, L.KV_FULL_RANGE if full_range else 0),
+                    "r4q_paged_kv_write")
 
 
 def paged_flash_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
@@ -572,36 +469,8 @@ def paged_flash_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     table are cut; ``check_status`` reports both.  The workspace comes from
     torch's allocator at every call, so calls on several streams and captured
     graphs share nothing."""
-    gpu = _same_gpu(q, k_pages, v_pages, block_table, seq_lens, k_scale, v_scale, out)
-    q, B, H, ldq = _heads(q, "q")
-    cache, Hk, page, nb = _paged_cache(k_pages, v_pages, block_table, k_scale, v_scale)
-    seq_lens = _vector(seq_lens, "seq_lens", torch.int64, B)
-    if out is None:
-        out, ldo = torch.empty(B, H, 128, dtype=torch.float16, device=q.device), H * 128
-    else:
-        out, _, _, ldo = _heads(out, "out", B, H, True)
-    need = _paged_workspace_bytes(gpu, B, H, Hk, page, nb)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _run_on(gpu, "r4q_paged_flash_decode", q.data_ptr(), ldq, cache, seq_lens.data_ptr(), out.data_ptr(), ldo, B, H,
-            L.ATTN_FWHT if fwht else 0, _ptr(ws), need)
-    return out
-
-
-def _host_ints(*lists) -> list:
-    """Host sequences or CPU tensors of equal length as arrays of C ints."""
-    out = []
-    for x in lists:
-        if isinstance(x, torch.Tensor):
-            if x.is_cuda:
-                raise ValueError("page lists are host data (lists or CPU tensors)")
-            x = x.tolist()
-        try:
-            out.append(array.array('i', x))
-        except OverflowError:
-            raise ValueError("page lists must hold 32-bit integers") from None
-        if len(out[-1]) != len(out[0]):
-            raise ValueError("page lists must have one length")
-    return out
+    return _checked(_native.paged_flash_decode(q, k_pages, v_pages, block_table, seq_lens, k_scale, v_scale,
+                                               L.ATTN_FWHT if fwht else 0, out), "r4q_paged_flash_decode")
 
 
 def kv_copy_pages(pool: torch.Tensor, src, dst) -> None:
@@ -610,28 +479,13 @@ def kv_copy_pages(pool: torch.Tensor, src, dst) -> None:
     [..., P, Hk, page, 128], contiguous; src and dst host lists.  A page may be
     copied to several places, but not written twice, nor both read and
     written (r4q_kv_copy_pages)."""
-    gpu = _same_gpu(pool)
-    if pool.dtype != torch.uint8 or pool.dim() < 4 or not pool.is_contiguous():
-        raise ValueError("pool must be uint8 [..., pages, kv heads, page, 128] and contiguous")
-    s, d = _host_ints(src, dst)
-    P = pool.shape[-4]
-    page_bytes = pool.shape[-3] * pool.shape[-2] * pool.shape[-1]
-    outer = pool.numel() // max(1, P * page_bytes)
-    if not pool.numel():
-        raise ValueError("empty pool")
-    _run_on(gpu, "r4q_kv_copy_pages", pool.data_ptr(), outer, P * page_bytes, page_bytes, page_bytes, P,
-            s.buffer_info()[0], d.buffer_info()[0], len(s))
+    _checked(_native.kv_copy_pages(pool, src, dst), "r4q_kv_copy_pages")
 
 
 def kv_table_set(table: torch.Tensor, rows, cols, values) -> None:
     """table[rows[i], cols[i]] = values[i] in stream order, from host lists
     (r4q_kv_table_set): table int32 [sequences, blocks] on the device; no cell twice."""
-    gpu = _same_gpu(table)
-    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError("table must be int32 [sequences, blocks] with contiguous rows")
-    r, c, v = _host_ints(rows, cols, values)
-    _run_on(gpu, "r4q_kv_table_set", table.data_ptr(), table.stride(0) if table.shape[0] > 1 else table.shape[1],
-            table.shape[0], table.shape[1], r.buffer_info()[0], c.buffer_info()[0], v.buffer_info()[0], len(r))
+    _checked(_native.kv_table_set(table, rows, cols, values), "r4q_kv_table_set")
 
 
 # ----------------------------------------------------------- token likelihoods ---
@@ -646,9 +500,6 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: torch.Tensor
 
 
-_LOGIT_TYPES = {torch.float16: L.T_F16, torch.bfloat16: L.T_BF16, torch.float32: L.T_F32}
-
-
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, k: int = 0) -> TokenLogprobs:
     """Log probabilities of ``tokens`` (int64 [M]) under softmax(logits[M, V])
     (fp16, bf16 or fp32; rows any stride apart), with their rank, the rows'
@@ -656,25 +507,4 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     logits (r4q_token_logprobs).  Ties go to the lowest id.  A token outside
     [0, V) gets NaN and rank 0; a row that is no distribution (NaN, +inf, or
     -inf throughout) gives NaN."""
-    ty = _LOGIT_TYPES.get(logits.dtype)
-    if ty is None:
-        raise TypeError(f"logits must be float16, bfloat16 or float32, not {logits.dtype}")
-    if logits.dim() != 2:
-        raise ValueError("logits must be [rows, vocabulary]")
-    gpu = _same_gpu(logits, tokens)
-    M, V = logits.shape
-    if V < 1 or not 0 <= k <= min(V, L.MAX_TOP):
-        raise ValueError(f"k must be in [0, {min(V, L.MAX_TOP)}], got {k} (vocabulary {V})")
-    ld, one = logits.stride()
-    if (one != 1 and V > 1) or (ld < V and M > 1):
-        logits, ld = logits.contiguous(), V
-    dev, logprob, rank = logits.device, None, None
-    entropy = torch.empty(M, dtype=torch.float32, device=dev)
-    if tokens is not None:
-        tokens = _vector(tokens, "tokens", torch.int64, M)
-        logprob, rank = torch.empty_like(entropy), torch.empty_like(tokens)
-    top_ids = torch.empty(M, k, dtype=torch.int64, device=dev)
-    top = torch.empty(M, k, dtype=torch.float32, device=dev)
-    _run_on(gpu, "r4q_token_logprobs", logits.data_ptr(), ty, ld if M > 1 else V, _ptr(tokens), M, V, k, _ptr(logprob),
-            _ptr(rank), entropy.data_ptr(), top_ids.data_ptr(), top.data_ptr())
-    return TokenLogprobs(logprob, rank, entropy, top_ids, top)
+    return TokenLogprobs(*_checked(_native.token_logprobs(logits, tokens, k), "r4q_token_logprobs"))

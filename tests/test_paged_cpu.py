@@ -219,11 +219,18 @@ def test_wrappers_take_cuda_tensors_only_and_host_lists():
                  lambda: ops.token_logprobs(k[0], pos, 1)):
         with pytest.raises(ValueError, match="CUDA"):
             call()
-    assert [list(x) for x in ops._host_ints([1, 2], torch.tensor([3, 4]))] == [[1, 2], [3, 4]]
-    with pytest.raises(ValueError):
-        ops._host_ints([1], [1, 2])
-    with pytest.raises(ValueError):
-        ops._host_ints([1 << 31])
+    for call in (lambda: ops.paged_flash_decode(None, pg, pg, t, pos), lambda: ops.kv_copy_pages([0], [0], [1]),
+                 lambda: ops.token_logprobs(3, pos, 1)):
+        with pytest.raises(TypeError, match="tensor"):
+            call()
+
+
+def test_native_module_formats_its_errors():
+    """Numbers in a message go through the C++ runtime's streams: they need the runtime that torch uses."""
+    with pytest.raises(TypeError, match="takes 9 arguments, got 1"):
+        ops._native.paged_flash_decode(1)
+    with pytest.raises(ValueError, match="null entry point"):
+        ops._native.bind(0, 0, 0, 0, 0, 0)
 
 
 class LogprobBackend:
@@ -266,6 +273,10 @@ def test_engine_collects_likelihoods_for_the_requests_that_want_them():
     for bad in (-1, 33):
         with pytest.raises(ValueError):
             eng.submit([1], logprobs=bad)
-    del LogprobBackend.logprobs
-    with pytest.raises(ValueError):
-        eng.submit([1], logprobs=1)
+
+
+def test_backend_without_likelihoods_refuses_them():
+    class Plain:
+        batch, max_seq = 1, 8
+    with pytest.raises(ValueError, match="log probabilities"):
+        serve.BatchedEngine(Plain()).submit([1], logprobs=1)
