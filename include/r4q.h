@@ -271,11 +271,11 @@ int r4q_paged_kv_write(const void* q, long ldq, const void* k, long ldk, const v
 /* o[b, h] = softmax(q[b,h]·K^T / sqrt(128)) V over positions [0, seq_lens[b])
  * of sequence b, as r4q_flash_decode over a contiguous cache (fp32 softmax and
  * sums, fp16 out, R4Q_ATTN_FWHT, zeros for an empty sequence).  B <= cache->seqs
- * rows; seq_lens int64 [B], device; any H that is a multiple of Hk.  A page id
+ * rows, 2048 at most; seq_lens int64 [B], device; any H that is a multiple of Hk.  A page id
  * outside the pool reads as zeros, a length beyond max_blocks * page is cut;
  * both are reported by r4q_kernel_status.  Bytes of a page behind the sequence
  * may hold anything.  workspace (16-byte aligned, of the size that
- * r4q_paged_flash_decode_workspace_bytes gives; may be 0, then NULL) needs no
+ * r4q_paged_flash_decode_workspace_bytes gives on this device; may be 0, then NULL) needs no
  * initialisation and keeps nothing between calls; calls that may run at once
  * need one each. */
 size_t r4q_paged_flash_decode_workspace_bytes(int B, int H, int Hk, int page, int max_blocks);

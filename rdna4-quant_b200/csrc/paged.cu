@@ -1,8 +1,8 @@
 // Paged FP8 KV cache: new tokens into pages (with the per-head RMSNorm + RoPE
 // of q and k), page copies over all layers, block-table updates, and the
 // status of the kernels that keep their status words in the library.
+#include <cstdlib>
 #include <cstring>
-#include <vector>
 
 #include "paged.cuh"
 #include "r4q_common.cuh"
@@ -16,13 +16,13 @@ __device__ int g_write_status;
 // A warp takes up to four heads of one kind (q, k or v) of one token, a half-warp
 // per head: what differs between the kinds is uniform in the warp, the token's
 // position, page and rotation row are looked up once, and eight loads a lane are
-// in flight together.  Lane s of a half holds
-// elements 2s, 2s + 1 of each 32-block: the RoPE partners i, i + 64 and the terms
-// that head_kernel (r4q_head_norm_rope) adds in one lane are in one lane here too,
-// and a butterfly over the half finishes the sum of squares in its order.  Norm
-// and rotation equal that kernel's to the bit, so a paged cache holds the bytes
-// that the contiguous one would.  Bound: issue slots (a warp per head took 184
-// instructions a head, mixed kinds in a warp 136).
+// in flight together.  Lane s of a half holds elements 2s, 2s + 1 of each
+// 32-block: the RoPE partners i, i + 64 and the terms that head_kernel
+// (r4q_head_norm_rope) adds in one lane are in one lane here too, and a butterfly
+// over the half finishes the sum of squares in its order.  Norm and rotation equal
+// that kernel's to the bit, so a paged cache holds the bytes that the contiguous
+// one would.  Bound: issue slots, 125 instructions a head (184 with a warp per
+// head, 136 with mixed kinds in a warp): 8192 tokens of 40/8 heads 72 us, 3.1 TB/s.
 constexpr int kPairs = 2;
 constexpr int kHeads = 2 * kPairs;
 struct WriteArgs {
@@ -306,18 +306,24 @@ extern "C" int r4q_kv_copy_pages(void* pool, long outer, long outer_stride, long
   const long chunks = (page_bytes / 16 + kCopyChunk - 1) / kCopyChunk;
   if (outer > 65535 || chunks > 0x7fffffffL)
     return set_error(R4Q_ERR_ARG, "kv_copy_pages: %ld pools (at most 65535) of %ld-byte pages", outer, page_bytes);
-  std::vector<uint8_t> seen(n ? n_pages : 0, 0);     // 1: read, 2: written
-  for (int i = 0; i < n; ++i) {
+  if (n == 0 || outer == 0) return R4Q_OK;
+  for (int i = 0; i < n; ++i)
     if (src[i] < 0 || src[i] >= n_pages || dst[i] < 0 || dst[i] >= n_pages)
       return set_error(R4Q_ERR_ARG, "kv_copy_pages: move %d (%d -> %d) outside the pool of %d pages", i, src[i],
                        dst[i], n_pages);
-    if (seen[dst[i]] & 2) return set_error(R4Q_ERR_ARG, "kv_copy_pages: page %d is written twice", dst[i]);
+  uint8_t* seen = (uint8_t*)calloc(n_pages, 1);      // per page, 1: read, 2: written
+  if (!seen) return set_error(R4Q_ERR_CAPACITY, "kv_copy_pages: no host memory for %d pages", n_pages);
+  int twice = -1, both = -1;
+  for (int i = 0; i < n; ++i) {
+    if (seen[dst[i]] & 2) twice = dst[i];
     seen[src[i]] |= 1;
     seen[dst[i]] |= 2;
   }
   for (int i = 0; i < n; ++i)
-    if (seen[src[i]] == 3) return set_error(R4Q_ERR_ARG, "kv_copy_pages: page %d is both read and written", src[i]);
-  if (n == 0 || outer == 0) return R4Q_OK;
+    if (seen[src[i]] == 3) both = src[i];
+  free(seen);
+  if (twice >= 0) return set_error(R4Q_ERR_ARG, "kv_copy_pages: page %d is written twice", twice);
+  if (both >= 0) return set_error(R4Q_ERR_ARG, "kv_copy_pages: page %d is both read and written", both);
   for (int at = 0; at < n; at += kMaxMoves) {
     const int part = n - at < kMaxMoves ? n - at : kMaxMoves;
     Moves mv;

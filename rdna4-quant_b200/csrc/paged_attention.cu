@@ -55,6 +55,7 @@ constexpr int kPartFloats = kGroup * kPitch;
 constexpr int kMaxBatch = 2048;
 constexpr int kJoinWarps = 4;
 constexpr int kWaitPolls = 1 << 22;
+constexpr float kLowest = -3e38f;                 // a maximum before the first score: no finite score is below it
 
 struct AttnArgs {
   const __half* q;
@@ -110,7 +111,7 @@ __device__ __forceinline__ void fwht32_x4(float (&v)[4], int lane) {
 
 // The running join of parts of a head, O 4 elements per lane.
 struct Joined {
-  float M = -1e30f, L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
+  float M = kLowest, L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
   __device__ __forceinline__ void add(float m, float l, const float4 v) {
     const float mn = fmaxf(M, m), f = ex2(M - mn), e = ex2(m - mn);
     M = mn;
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     look_up(beg);
     uint32_t qa[8], qb[8];
-    float m = -1e30f, l = 0.f, scale = 0.f, oacc[16][4];
+    float m = kLowest, l = 0.f, scale = 0.f, oacc[16][4];
     int seq = 0;
     bool first = at.t == 0;                                   // the segment began in this warp
     auto start_segment = [&]() {
@@ -313,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint4 v = head < a.Hg ? qp[i] : make_uint4(0, 0, 0, 0);
         qa[2 * i] = v.x; qb[2 * i] = v.y; qa[2 * i + 1] = v.z; qb[2 * i + 1] = v.w;
       }
-      m = -1e30f;
+      m = kLowest;
       l = 0.f;
 #pragma unroll
       for (int j = 0; j < 16; ++j)

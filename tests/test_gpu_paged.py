@@ -137,6 +137,21 @@ def test_attention_large_scores_and_spread():
     check_attention(o, *ref_attention(q, kp, vp, table, lens, None, None, False))
 
 
+def test_attention_scores_of_any_finite_size():
+    """All scores alike, at -1e31 and at +1e31: the plain mean of V (a bound that a mask value could be mistaken for)."""
+    from r4q import ops
+    kp, vp, table, _, _ = make_paged([70], 1, 16, seed=12)
+    kp[table[0, :5].long()] = 0x38                    # 1.0
+    sc = torch.tensor([1e30], device="cuda")
+    ids = table[0, :5].long()
+    mean = decode_lut()[vp[ids, 0].reshape(-1, D)[:70].long()]
+    for sign in (-1.0, 1.0):
+        q = torch.full((1, 8, D), sign, device="cuda").half()
+        o = ops.paged_flash_decode(q, kp, vp, table, torch.tensor([70], device="cuda"), k_scale=sc)
+        tol = mean.abs().mean(0) * (2.0 ** -20 + 80 * U) + mean.mean(0).abs() * 2.0 ** -11 + 2.0 ** -25
+        assert ((o[0].double() - mean.mean(0)).abs() <= tol).all()
+
+
 def test_attention_views_strides_and_shared_pages():
     """q out of a wider row, K and V interleaved in one pool, a table with wider rows and more of them than the
     batch, an output with its own stride; two sequences on the same pages give the same result."""
@@ -207,6 +222,38 @@ def test_attention_streams_and_graphs_share_nothing():
     torch.cuda.synchronize()
     check_attention(outs[0], *ref_attention(qs[0], *sets[0][:3], [0, 10, 100], None, None, False))
     ops.check_status()
+
+
+def test_first_call_may_be_captured(tmp_path):
+    """In a fresh process, all operators for the first time under capture: nothing has to be warmed up."""
+    import subprocess
+    import sys
+    from conftest import PKG
+    code = f"""
+import sys; sys.path.insert(0, {str(PKG)!r})
+import torch
+from r4q import ops
+z = lambda *s, dtype=torch.uint8: torch.zeros(*s, dtype=dtype, device="cuda")
+pool, table, k = z(1, 2, 64, 2, 16, 128), torch.arange(60, dtype=torch.int32, device="cuda").view(2, 30), z(2, 2, 128, dtype=torch.half)
+pos, x = torch.tensor([0, 400], device="cuda"), torch.randn(3, 9000, device="cuda").half()
+k += 1
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    ops.paged_kv_write(k, k, pool[0, 0], pool[0, 1], table, pos)
+    o = ops.paged_flash_decode(k, pool[0, 0], pool[0, 1], table, pos + 1)
+    ops.kv_copy_pages(pool, [0], [63])
+    ops.kv_table_set(table, [1], [29], [63])
+    r = ops.token_logprobs(x, x.argmax(-1), 4)
+g.replay()
+torch.cuda.synchronize()
+ops.check_status()
+assert (o[0] == 1).all() and torch.isfinite(o).all() and (r.rank == 1).all()
+assert torch.equal(pool[:, :, 63], pool[:, :, 0]) and pool[0, 0, 0].any() and table[1, 29] == 63
+print("captured")
+"""
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
 
 
 def test_attention_reports_bad_pages_and_lengths():
