@@ -310,7 +310,9 @@ enum { R4Q_T_F16 = 0, R4Q_T_BF16 = 1, R4Q_T_F32 = 2 };
  * over one pass.  tokens int64 [M] (NULL: only entropy and top); an id outside
  * [0, V) gets logprob NaN and rank 0.  A row with NaN or +inf, or with nothing
  * above -inf, has no distribution: its log probabilities and entropy are NaN
- * (NaN counts as the lowest value in the order).  Outputs may be NULL.
+ * (NaN counts as the lowest value in the order).  Outputs may be NULL.  The
+ * order of the sums goes by M, V and the rows' alignment: equal calls give equal
+ * bits, another number of rows may round otherwise.
  * The reference returns no likelihoods (api_server.py:58-150). */
 int r4q_token_logprobs(const void* logits, int type, long ld, const long long* tokens, int M, int V, int k,
                        float* logprob, long long* rank, float* entropy, long long* top_ids, float* top_logprobs,

@@ -159,6 +159,27 @@ def test_strides_and_alignment():
         check(big.t()[:3000].t(), t % 3000, 6)
 
 
+def test_rows_beyond_32_bit_offsets_and_grids():
+    """Rows whose first element lies beyond 2^31, and more rows than a grid dimension takes."""
+    from r4q import ops
+    V = 1 << 20
+    x = torch.zeros(2100, V, dtype=torch.float16, device="cuda")
+    big, t = logits(3, V, torch.float16, 7)
+    x[-3:] = big
+    t = torch.cat([torch.zeros(2097, dtype=torch.int64, device="cuda"), t])
+    r = ops.token_logprobs(x, t, 3)
+    few = check(big, t[-3:], 3)
+    # the sums run in an order that goes by the number of rows, so both lie within the bound of the exact value
+    # (here |x_t - m| and log S below 32): twice that of each other; ids and ranks are equal
+    assert torch.equal(r.rank[-3:], few.rank) and torch.equal(r.top_ids[-3:], few.top_ids)
+    for a, b, tol in ((r.logprob, few.logprob, 1), (r.top_logprobs, few.top_logprobs, 1), (r.entropy, few.entropy, 64)):
+        assert ((a[-3:] - b).abs() <= 2 * tol * (2.0 ** -18 + 2 * U * 64)).all()
+    assert (r.rank[:2097] == 1).all() and torch.equal(r.top_ids[:2097], torch.arange(3, device="cuda").expand(2097, 3))
+    del x, r
+    many, t = logits(70000, 40, torch.float32, 8)
+    check(many, t, 2)
+
+
 def test_repeatable_streams_and_graphs():
     from r4q import ops
     sets = [logits(5, 151936, torch.float16, 31), logits(300, 32003, torch.bfloat16, 32)]

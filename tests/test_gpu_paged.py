@@ -511,6 +511,29 @@ def test_wrapper_refusals_on_device_tensors():
             pytest.fail(f"call {i} was accepted")
 
 
+def test_pools_beyond_32_bit_offsets():
+    """5 GB each of K and V in one interleaved pool, the used pages at both ends: write, attention, copy."""
+    from r4q import ops
+    Hk, page, P = 8, 64, 80000
+    pool = torch.zeros(2, P, Hk, page, D, dtype=torch.uint8, device="cuda")
+    g = torch.Generator("cuda").manual_seed(3)
+    n = 150
+    table = torch.tensor([[P - 1, 0, P - 7], [1, P // 2, 2]], dtype=torch.int32, device="cuda")
+    lens = [n, 70]
+    k, v = (torch.randn(sum(lens), Hk, D, generator=g, device="cuda").half() for _ in range(2))
+    pos = torch.cat([torch.arange(m) for m in lens]).cuda()
+    rows = torch.cat([torch.full((m,), i) for i, m in enumerate(lens)]).int().cuda()
+    ops.paged_kv_write(k, v, pool[0], pool[1], table, pos, rows=rows)
+    q = torch.randn(2, 16, D, generator=g, device="cuda").half()
+    seq = torch.tensor(lens, device="cuda")
+    o = ops.paged_flash_decode(q, pool[0], pool[1], table, seq)
+    check_attention(o, *ref_attention(q, pool[0], pool[1], table, lens, None, None, False))
+    ops.kv_copy_pages(pool, [P - 1, P - 7], [P - 2, 3])
+    ops.kv_table_set(table, [0, 0], [0, 2], [P - 2, 3])
+    assert torch.equal(ops.paged_flash_decode(q, pool[0], pool[1], table, seq), o)
+    ops.check_status()
+
+
 # ------------------------------------------------------------- used together ---
 def test_cache_life_prefix_forks_copies_compaction():
     """Sequences prefilled, forked, extended (a shared page is copied before it is written), freed and compacted;
