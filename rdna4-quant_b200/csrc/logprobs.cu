@@ -38,6 +38,7 @@
 #include <mutex>
 #include <type_traits>
 
+#include "f32x2.cuh"
 #include "paged.cuh"
 #include "r4q_common.cuh"
 #include "tma_dev.cuh"
@@ -64,33 +65,6 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-// two fp32 operations an instruction
-struct F2 {
-  uint64_t v;
-  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
-  __device__ __forceinline__ explicit F2(uint64_t u) : v(u) {}
-  __device__ __forceinline__ float2 get() const {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-    return f;
-  }
-};
-__device__ __forceinline__ F2 add(F2 a, F2 b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
-  return F2(d);
-}
-__device__ __forceinline__ F2 mul(F2 a, F2 b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
-  return F2(d);
-}
-__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return F2(d);
 }
 
 // order of floats as unsigned integers; NaN is the lowest, -0 equals +0

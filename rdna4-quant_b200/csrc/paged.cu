@@ -4,6 +4,7 @@
 #include <cstdlib>
 #include <cstring>
 
+#include "f32x2.cuh"
 #include "paged.cuh"
 #include "r4q_common.cuh"
 
@@ -21,8 +22,9 @@ __device__ int g_write_status;
 // (r4q_head_norm_rope) adds in one lane are in one lane here too, and a butterfly
 // over the half finishes the sum of squares in its order.  Norm and rotation equal
 // that kernel's to the bit, so a paged cache holds the bytes that the contiguous
-// one would.  Bound: issue slots, 125 instructions a head (184 with a warp per
-// head, 136 with mixed kinds in a warp): 8192 tokens of 40/8 heads 72 us, 3.1 TB/s.
+// one would.  Bound: issue slots, so the arithmetic is two-wide fp32: 8192 tokens
+// of 40/8 heads 60 us, 3.6 TB/s (72 us with scalar fp32 and comparisons per value;
+// a warp per head, 4 bytes a lane, 92).
 constexpr int kPairs = 2;
 constexpr int kHeads = 2 * kPairs;
 struct WriteArgs {
@@ -41,29 +43,36 @@ struct WriteArgs {
   int flags;
 };
 
-// The value that the cache codec (fp8_encode) stores for x: three mantissa bits,
-// ties away from zero, a signed zero below 2^-6, and 448 from 256 on, or with
-// `full` for what exceeds it only.  The hardware conversion of such a value is
-// exact, so rounding on the float and converting in pairs gives fp8_encode's
-// bytes in half its instructions.
-__device__ __forceinline__ float stored(float x, bool full) {
-  const uint32_t u = __float_as_uint(fmaxf(-448.0f, fminf(448.0f, x)));
-  const float r = __uint_as_float((u + 0x80000u) & 0xfff00000u);
-  const float top = !full && fabsf(r) >= 256.0f ? 448.0f : fabsf(r);
-  return copysignf(fabsf(r) < 0x1p-6f ? 0.0f : top, r);
+// The codes of four values.  The cache codec (fp8_encode) keeps three mantissa
+// bits, ties away from zero; below 2^-6 it keeps the sign alone, and from 256 on
+// (with `full`: from 448 on) it stores 448, which it also stores for NaN.  Here the
+// rounding is done on the float, so that the hardware's conversion in pairs is
+// exact; 2^-6 is the smallest normal number at a scale of 2^-120, below which the
+// fp32 pipe flushes to a signed zero; and the top binade is set to 448 on four
+// bytes at once.  Five integer instructions a value: that pipe is what bounds a
+// plain write (a dozen with comparisons and selections on each float).
+__device__ __forceinline__ float rounded(float x) {
+  const uint32_t u = __float_as_uint(fminf(x, 448.0f));                 // NaN: 448; the conversion bounds the other side
+  float r = __uint_as_float((u + 0x80000u) & 0xfff00000u);
+  asm("mul.rn.ftz.f32 %0, %0, 0f03800000;" : "+f"(r));                  // 2^-120
+  return r * 0x1p120f;
 }
-__device__ __forceinline__ uint32_t encode2(float a, float b, const float* scale, int kh, bool full) {
-  if (scale) {
-    const float s = scale[kh];
-    a = a / s;
-    b = b / s;
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, bool full) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(rounded(b)), "f"(rounded(a)));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(rounded(d)), "f"(rounded(c)));
+  uint32_t w = (uint32_t)lo | (uint32_t)hi << 16;
+  if (!full) {
+    const uint32_t top = ((w & 0x78787878u) + 0x08080808u) & 0x80808080u, one = top >> 7;   // exponent field 15
+    w = (w | (top - one)) & ~one;
   }
-  uint16_t d;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(stored(b, full)), "f"(stored(a, full)));
-  return d;
+  return w;
 }
 
-__device__ __forceinline__ float2 half2_of(uint32_t u) { return __half22float2(u32_as_h2(u)); }
+__device__ __forceinline__ F2 pair_of(uint32_t u) {
+  const float2 f = __half22float2(u32_as_h2(u));
+  return F2(f.x, f.y);
+}
 
 __global__ void __launch_bounds__(256) paged_write_kernel(const WriteArgs a) {
   const int lane = threadIdx.x & 31, sl = lane & 15, half = lane >> 4;
@@ -91,7 +100,7 @@ __global__ void __launch_bounds__(256) paged_write_kernel(const WriteArgs a) {
   bool ok = row >= 0 && row < a.c.seqs && pos < (long long)a.c.max_blocks * a.c.page;
   if (ok && (a.flags & R4Q_HEAD_ROPE)) ok = pos < a.tab_rows;   // of a token, all heads or none
   int pg = 0, in_page = 0;
-  float2 c[2] = {{1.f, 1.f}, {1.f, 1.f}}, s[2] = {{0.f, 0.f}, {0.f, 0.f}};
+  uint32_t c32[2] = {0u, 0u}, s32[2] = {0u, 0u};
   if (ok) {
     const int blk = a.by_page.div((int)pos);
     in_page = (int)pos - blk * a.c.page;
@@ -99,8 +108,8 @@ __global__ void __launch_bounds__(256) paged_write_kernel(const WriteArgs a) {
     if (rope)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        c[j] = half2_of(reinterpret_cast<const uint32_t*>(a.cos_tab + pos * a.tab_stride)[sl + 16 * j]);
-        s[j] = half2_of(reinterpret_cast<const uint32_t*>(a.sin_tab + pos * a.tab_stride)[sl + 16 * j]);
+        c32[j] = reinterpret_cast<const uint32_t*>(a.cos_tab + pos * a.tab_stride)[sl + 16 * j];
+        s32[j] = reinterpret_cast<const uint32_t*>(a.sin_tab + pos * a.tab_stride)[sl + 16 * j];
       }
     ok = pg >= 0 && pg < a.c.n_pages;
   }
@@ -122,52 +131,48 @@ __global__ void __launch_bounds__(256) paged_write_kernel(const WriteArgs a) {
   for (int i = 0; i < kPairs; ++i) {
     if (2 * i >= n) break;                           // uniform
     const bool in = 2 * i + half < n;
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = half2_of(x32[i][j]);
-      v[2 * j] = f.x;
-      v[2 * j + 1] = f.y;
-    }
+    F2 v[4] = {pair_of(x32[i][0]), pair_of(x32[i][1]), pair_of(x32[i][2]), pair_of(x32[i][3])};
     if (norm) {
-      float s0 = 0.f, s1 = 0.f;
+      F2 ss(0.f, 0.f);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s0 += v[2 * j] * v[2 * j];
-        s1 += v[2 * j + 1] * v[2 * j + 1];
-      }
+      for (int j = 0; j < 4; ++j) ss = fma(v[j], v[j], ss);
 #pragma unroll
       for (int d = 8; d > 0; d >>= 1) {
-        s0 += __shfl_xor_sync(0xffffffffu, s0, d);
-        s1 += __shfl_xor_sync(0xffffffffu, s1, d);
+        const float2 f = ss.get();
+        ss = add(ss, F2(__shfl_xor_sync(0xffffffffu, f.x, d), __shfl_xor_sync(0xffffffffu, f.y, d)));
       }
-      const float rrms = rsqrtf((s0 + s1) / (float)kHeadDim + a.eps);
+      const float2 f = ss.get();
+      const float rrms = rsqrtf((f.x + f.y) / (float)kHeadDim + a.eps);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = half2_of(w32[j]);
-        v[2 * j] = v[2 * j] * rrms * f.x;
-        v[2 * j + 1] = v[2 * j + 1] * rrms * f.y;
-      }
+      for (int j = 0; j < 4; ++j) v[j] = mul(mul(v[j], F2(rrms, rrms)), pair_of(w32[j]));
     }
     if (rope)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float e0 = v[2 * j], o0 = v[2 * j + 4], e1 = v[2 * j + 1], o1 = v[2 * j + 5];
-        v[2 * j] = e0 * c[j].x - o0 * s[j].x;
-        v[2 * j + 4] = o0 * c[j].x + e0 * s[j].x;
-        v[2 * j + 1] = e1 * c[j].y - o1 * s[j].y;
-        v[2 * j + 5] = o1 * c[j].y + e1 * s[j].y;
+        const F2 e = v[j], o = v[j + 2], c = pair_of(c32[j]);
+        const F2 s = pair_of(s32[j]), minus_s = pair_of(s32[j] ^ 0x80008000u);
+        v[j] = fma(e, c, mul(o, minus_s));
+        v[j + 2] = fma(o, c, mul(e, s));
       }
+    float2 f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = v[j].get();
     if (out && in)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        o32[i * kHeadDim + 16 * j] = h2_as_u32(__floats2half2_rn(v[2 * j], v[2 * j + 1]));
+      for (int j = 0; j < 4; ++j) o32[i * kHeadDim + 16 * j] = h2_as_u32(__floats2half2_rn(f[j].x, f[j].y));
     if (is_q) continue;
     // a lane has the codes of elements 2s, 2s + 1 of four 32-blocks: even lanes
     // store four bytes of blocks 0 and 1 with their neighbour's, odd lanes of 2 and 3
-    const int kh = min(h0 + 2 * i + half, a.c.Hk - 1);
-    const uint32_t e01 = encode2(v[0], v[1], scale, kh, full) | encode2(v[2], v[3], scale, kh, full) << 16;
-    const uint32_t e23 = encode2(v[4], v[5], scale, kh, full) | encode2(v[6], v[7], scale, kh, full) << 16;
+    if (scale) {
+      const float s = scale[min(h0 + 2 * i + half, a.c.Hk - 1)];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[j].x = f[j].x / s;
+        f[j].y = f[j].y / s;
+      }
+    }
+    const uint32_t e01 = encode4(f[0].x, f[0].y, f[1].x, f[1].y, full);
+    const uint32_t e23 = encode4(f[2].x, f[2].y, f[3].x, f[3].y, full);
     const bool even = !(lane & 1);
     const uint32_t own = even ? e01 : e23, got = __shfl_xor_sync(0xffffffffu, even ? e23 : e01, 1);
     if (in) {
