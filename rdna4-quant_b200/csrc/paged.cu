@@ -26,6 +26,7 @@ __device__ int g_write_status;
 // of 40/8 heads 60 us, 3.6 TB/s (72 us with scalar fp32 and comparisons per value;
 // a warp per head, 4 bytes a lane, 92).
 constexpr int kPairs = 2;
+constexpr int kWriteThreads = 128;
 constexpr int kHeads = 2 * kPairs;
 struct WriteArgs {
   const __half *q, *k, *v;
@@ -74,7 +75,7 @@ __device__ __forceinline__ F2 pair_of(uint32_t u) {
   return F2(f.x, f.y);
 }
 
-__global__ void __launch_bounds__(256) paged_write_kernel(const WriteArgs a) {
+__global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const WriteArgs a) {
   const int lane = threadIdx.x & 31, sl = lane & 15, half = lane >> 4;
   const int w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const int m = a.by_groups.div(w);
@@ -292,7 +293,8 @@ extern "C" int r4q_paged_kv_write(const void* q, long ldq, const void* k, long l
   const long warps = (long)M * a.groups;
   if (warps > 0x7ffffff0L) return set_error(R4Q_ERR_ARG, "paged_kv_write: %d tokens of %d heads are too many", M, H);
   const cudaError_t e =
-      launch_pdl(paged_write_kernel, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, (cudaStream_t)stream, a);
+      launch_pdl(paged_write_kernel, dim3((unsigned)((warps * 32 + kWriteThreads - 1) / kWriteThreads)),
+                 dim3(kWriteThreads), 0, (cudaStream_t)stream, a);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return set_error(R4Q_ERR_CUDA, "paged_write_kernel: %s", cudaGetErrorString(e));
