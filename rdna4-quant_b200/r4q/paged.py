@@ -8,7 +8,7 @@ and block-table cells that each operation calls for.  ``PagedKVCache`` holds
 the pages of all layers and the block table on the GPU and carries those plans
 out with ``ops.kv_copy_pages`` / ``ops.kv_table_set`` on the current stream.
 The reference keeps one contiguous cache per request
-(int4_engine_v5.py:129-175) and has no counterpart."""
+(api_server.py:58-150) and has no counterpart."""
 from __future__ import annotations
 
 from dataclasses import dataclass, field
@@ -119,9 +119,18 @@ class PageAllocator:
             self.lengths[s] = end
         return plan
 
+    def check_writable(self, seq: int, end: int) -> None:
+        """ValueError unless the sequence holds positions [0, end) on pages that no other one shares."""
+        if self.lengths[self._seq(seq)] < end:
+            raise ValueError(f"sequence {seq} holds {self.lengths[seq]} positions, not {end}")
+        shared = [p for p in self.blocks[seq][:-(-end // self.page)] if self.refs[p] > 1]
+        if shared:
+            raise ValueError(f"sequence {seq} shares pages {shared[:4]} with another one")
+
     def fork(self, parent: int, child: int, length: Optional[int] = None) -> Plan:
         """The empty sequence ``child`` gets the first ``length`` positions of
-        ``parent`` (default: all), by sharing their pages."""
+        ``parent`` (default: all, also those reserved and not written yet), by
+        sharing their pages."""
         self._seq(parent)
         self._seq(child)
         length = self.lengths[parent] if length is None else int(length)

@@ -75,9 +75,9 @@ def prefill_logits(hidden: torch.Tensor, qkv_w, qkv_s, o_w, o_s, gu_w, gu_s, dow
     qkv_n = qd + 2 * kvd
     pos = torch.arange(M, dtype=torch.int64, device=dev)
     if pages is not None:
-        if pages.lengths[batch_row] < M or rope_cos.shape[0] < M:
-            raise ValueError(f"sequence {batch_row} holds {pages.lengths[batch_row]} positions and the RoPE tables "
-                             f"{rope_cos.shape[0]}, the prompt {M}")
+        pages.alloc.check_writable(int(batch_row), M)
+        if rope_cos.shape[0] < M:
+            raise ValueError(f"a prompt of {M} tokens for {rope_cos.shape[0]} rows of the RoPE tables")
         rows = torch.full((M,), int(batch_row), dtype=torch.int32, device=dev)
     normed = ops.rmsnorm(x, in_norm_w[0], rms_eps)
     nl = len(qkv_w)

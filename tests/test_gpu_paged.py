@@ -676,6 +676,10 @@ def test_prefill_into_pages_then_decode_attention():
     with pytest.raises(ValueError):
         P.prefill_logits(*args, pages=pages, batch_row=1)
     pages.extend({1: 45})
+    pages.fork(1, 2, 10)
+    with pytest.raises(ValueError, match="shares"):
+        P.prefill_logits(*args, pages=pages, batch_row=1)
+    pages.free(2)
     b = P.prefill_logits(*args, pages=pages, batch_row=1, last_only=True)
     close(b.float().cpu().numpy(), a.float().cpu().numpy(), 5e-3)
     lut = decode_lut()

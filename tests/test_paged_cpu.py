@@ -95,6 +95,19 @@ def test_two_forks_writing_one_page_copy_it_once():
     assert (plan.src, plan.dst, a.refs[:2]) == ([0], [1], [1, 1])
 
 
+def test_check_writable():
+    a = paged.PageAllocator(8, 16, 3, 4)
+    a.extend({0: 40})
+    a.check_writable(0, 40)
+    a.fork(0, 1, 20)
+    for seq, end in ((0, 41), (0, 1), (1, 20), (3, 1), (-1, 1)):
+        with pytest.raises(ValueError):
+            a.check_writable(seq, end)
+    a.check_writable(2, 0)
+    a.free(0)
+    a.check_writable(1, 20)
+
+
 def test_allocator_refusals():
     a = paged.PageAllocator(4, 16, 3, 2)
     a.extend({0: 20})
