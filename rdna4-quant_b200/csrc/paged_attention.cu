@@ -15,8 +15,8 @@
 // device.  Every CTA takes an equal run of it and every warp of the CTA an equal
 // run of that, whatever the lengths are: a batch of one long and many short
 // sequences loads the SMs as evenly as an even one.  A (sequence, head) that lies
-// inside one warp's run is finished in its registers; parts join in shared
-// memory within a CTA, and through the workspace across CTAs, in a second small
+// inside one warp's run is finished by that warp; parts join in shared memory
+// within a CTA, and through the workspace across CTAs, in a second small
 // kernel (programmatic dependent launch) that reads them in list order: no
 // atomics and no state between calls, so results repeat bit for bit and nothing
 // is shared by calls that run at once.
@@ -435,41 +435,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         const int kh = a.by_chunks.div(at.hc), hg = (at.hc - kh * a.chunks) * kGroup + g;
-        if (first && last) {                                  // whole: lane holds elements 32 t .. 32 t + 31 of head g
-          float v[32];
-          const float inv = l > 0.f ? (a.c.v_scale ? a.c.v_scale[kh] : 1.f) / l : 0.f;
+        // head: began before, ends here; tail: goes on in the next warp; a whole one passes through the tail's place
+        const int which = last && !first ? 0 : 1;
+        float* p = part0 + (2 * warp + which) * kPartFloats + g * kPitch;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            v[j] = (oacc[j][0] + oacc[j][2]) * inv;
-            v[16 + j] = (oacc[j][1] + oacc[j][3]) * inv;
+        for (int j = 0; j < 16; j += 4) {
+          *reinterpret_cast<float4*>(p + 32 * t + j) =
+              make_float4(oacc[j][0] + oacc[j][2], oacc[j + 1][0] + oacc[j + 1][2], oacc[j + 2][0] + oacc[j + 2][2],
+                          oacc[j + 3][0] + oacc[j + 3][2]);
+          *reinterpret_cast<float4*>(p + 32 * t + 16 + j) =
+              make_float4(oacc[j][1] + oacc[j][3], oacc[j + 1][1] + oacc[j + 1][3], oacc[j + 2][1] + oacc[j + 2][3],
+                          oacc[j + 3][1] + oacc[j + 3][3]);
+        }
+        if (t == 0) {
+          p[kHeadDim] = m;
+          p[kHeadDim + 1] = l;
+        }
+        if (first && last) {
+          __syncwarp();
+          const float* part = part0 + (2 * warp + 1) * kPartFloats;
+#pragma unroll 1
+          for (int h = 0; h < kGroup && hg - g + h < a.Hg; ++h) {
+            const float4 v = *reinterpret_cast<const float4*>(part + h * kPitch + 4 * lane);
+            float O[4] = {v.x, v.y, v.z, v.w};
+            store_head(a, out_head(a, at.b, kh * a.Hg + hg - g + h), kh, part[h * kPitch + kHeadDim + 1], O, lane);
           }
-          if (a.fwht) fwht32_regs(v);
-          if (hg < a.Hg) {
-            uint4* dst = reinterpret_cast<uint4*>(a.o + (long)at.b * a.ldo + ((long)kh * a.Hg + hg) * kHeadDim + 32 * t);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              dst[i] = make_uint4(h2_as_u32(__floats2half2_rn(v[8 * i], v[8 * i + 1])),
-                                  h2_as_u32(__floats2half2_rn(v[8 * i + 2], v[8 * i + 3])),
-                                  h2_as_u32(__floats2half2_rn(v[8 * i + 4], v[8 * i + 5])),
-                                  h2_as_u32(__floats2half2_rn(v[8 * i + 6], v[8 * i + 7])));
-          }
-        } else {
-          const int which = last ? 0 : 1;                     // head: ends here; tail: goes on in the next warp
-          float* p = part0 + (2 * warp + which) * kPartFloats + g * kPitch;
-#pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            *reinterpret_cast<float4*>(p + 32 * t + j) =
-                make_float4(oacc[j][0] + oacc[j][2], oacc[j + 1][0] + oacc[j + 1][2], oacc[j + 2][0] + oacc[j + 2][2],
-                            oacc[j + 3][0] + oacc[j + 3][2]);
-            *reinterpret_cast<float4*>(p + 32 * t + 16 + j) =
-                make_float4(oacc[j][1] + oacc[j][3], oacc[j + 1][1] + oacc[j + 1][3], oacc[j + 2][1] + oacc[j + 2][3],
-                            oacc[j + 3][1] + oacc[j + 3][3]);
-          }
-          if (t == 0) {
-            p[kHeadDim] = m;
-            p[kHeadDim + 1] = l;
-          }
-          if (lane == 0) meta[2 * warp + which] = at.b * Hc + at.hc;
+          __syncwarp();
+        } else if (lane == 0) {
+          meta[2 * warp + which] = at.b * Hc + at.hc;
         }
         if (x + 1 < end) {                                    // the next segment
           at.t = 0;
