@@ -30,7 +30,9 @@
 // Precision.  q, K and V enter the products exactly (f16); a weight enters as
 // two f16 numbers, its rounding and what that left, which takes no extra
 // instruction: query heads fill 8 of the 16 rows of a product, the remainders the
-// other 8.  Scores, maxima, sums and O are fp32.  One rounding to f16 at the end.
+// other 8.  Weights are carried times 2^15 (l too, so that it cancels): f16 then
+// holds them to 2^-22 of themselves down to 2^-18 of the largest, and to 2^-40 of
+// that below.  Scores, maxima, sums and O are fp32.  One rounding to f16 at the end.
 #include <cuda.h>
 
 #include <mutex>
@@ -55,6 +57,7 @@ constexpr int kPartFloats = kGroup * kPitch;
 constexpr int kMaxBatch = 2048;
 constexpr int kJoinWarps = 4;
 constexpr int kWaitPolls = 1 << 22;
+constexpr float kWeightBits = 15.f;               // weights are carried times 2^15
 constexpr float kLowest = -3e38f;                 // a maximum before the first score: no finite score is below it
 
 struct AttnArgs {
@@ -389,9 +392,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 4; ++i) oacc[j][i] *= f;
       }
       uint32_t ph[4], pl[4];                                  // rounded weights and remainders
+      const float base = m - kWeightBits;
 #pragma unroll
       for (int nt = 0; nt < 4; ++nt) {
-        const float e0 = ex2(sc[nt][0] - m), e1 = ex2(sc[nt][1] - m);
+        const float e0 = ex2(sc[nt][0] - base), e1 = ex2(sc[nt][1] - base);
         l += e0 + e1;
         const __half2 h = __floats2half2_rn(e0, e1);
         const float2 r = __half22float2(h);

@@ -12,7 +12,10 @@ fp16: half a step is 2^-11 relative, 2^-25 below the normal range):
   sum |q k|; weights are e^(score), so off by twice that (numerator and sum),
   plus 2^-21 for the exponential and 2^-21 for carrying a weight as a pair of
   fp16 numbers, plus (64 + n/8) u for sums over n positions on tensor cores;
-  all of it times sum p |v|, then the rounding.  The H32 transform adds 32
+  all of it times sum p |v|.  A pair ends at 2^-40 of the largest weight (an fp16
+  step of 2^-24, halved, of weights carried times 2^15), whatever its own weight
+  is: 2^-40 sum |v| / sum e, with sum e >= 1 the weights relative to the largest.
+  Then the rounding.  The H32 transform adds 32
   such errors and divides by sqrt(32), with 6 u of its own."""
 import numpy as np
 import pytest
@@ -79,7 +82,7 @@ def ref_attention(q, kp, vp, table, lens, ks, vs, fwht):
             p = torch.softmax(qq @ K.t(), -1)
             err = 2 * 128 * U * (qq.abs() @ K.abs().t()).amax(-1) + 2.0 ** -20 + (64 + n / 8) * U
             out[b, h * Hg:(h + 1) * Hg] = p @ Vv
-            tol[b, h * Hg:(h + 1) * Hg] = err[:, None] * (p @ Vv.abs())
+            tol[b, h * Hg:(h + 1) * Hg] = err[:, None] * (p @ Vv.abs()) + 2.0 ** -40 * Vv.abs().sum(0)
     if fwht:
         hm = torch.from_numpy(O.hadamard_matrix(32).astype(np.float64)).cuda()
         hm = hm / hm[0].norm()
@@ -135,6 +138,22 @@ def test_attention_large_scores_and_spread():
     q = (torch.randn(2, 8, D, generator=torch.Generator("cuda").manual_seed(2), device="cuda") * 20).half()
     o = ops.paged_flash_decode(q, kp, vp, table, torch.tensor(lens, device="cuda"))
     check_attention(o, *ref_attention(q, kp, vp, table, lens, None, None, False))
+
+
+def test_attention_small_weights_keep_their_digits():
+    """One position takes nearly all the weight and has V = 0: what comes out is the sum of weights around 2^-22."""
+    from r4q import ops
+    n = 300
+    kp, vp, table, _, _ = make_paged([n], 1, 16, seed=15, std=0.3)
+    first = table[0, 0].long()
+    kp[first, 0, 0], vp[first, 0, 0] = 0, 0
+    kp[first, 0, 0, 0] = 0x58                         # 16.0
+    q = torch.zeros(1, 8, D, device="cuda").half()
+    q[:, :, 0] = 10.75 + 0.01 * torch.arange(8, device="cuda")
+    o = ops.paged_flash_decode(q, kp, vp, table, torch.tensor([n], device="cuda"))
+    ref, tol = ref_attention(q, kp, vp, table, [n], None, None, False)
+    assert ref.abs().max() < 1e-4
+    check_attention(o, ref, tol)
 
 
 def test_attention_scores_of_any_finite_size():
