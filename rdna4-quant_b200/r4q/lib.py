@@ -8,7 +8,6 @@ from __future__ import annotations
 
 import ctypes as C
 import os
-import struct
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent.parent
@@ -63,10 +62,6 @@ class ModelDesc(C.Structure):
         ("lm_w", C.c_void_p), ("lm_s", C.c_void_p), ("lm_n", C.c_int), ("tp_rank", C.c_int),
         ("tp_size", C.c_int), ("comm", C.c_void_p)]
 
-
-# r4q_paged_cache (include/r4q.h) in the platform's C layout: k_pages, v_pages, k_stride, v_stride, n_pages, page, Hk,
-# table, ld_table, seqs, max_blocks, k_scale, v_scale (0: NULL); the packed bytes are passed as the pointer
-PAGED_CACHE = struct.Struct("@PPlliiiPliiPP")
 
 _SIGS = {
     "r4q_last_error": (C.c_char_p, []),
@@ -158,6 +153,4 @@ W_INT4, W_INT8, W_FP16 = 0, 1, 2
 HEAD_NORM, HEAD_ROPE, HEAD_KV = 1, 2, 4
 KV_FULL_RANGE = 8
 ATTN_FWHT = 1
-# element types of r4q_token_logprobs
-T_F16, T_BF16, T_F32 = 0, 1, 2
-MAX_TOP = 32
+MAX_TOP = 32          # most alternatives of r4q_token_logprobs

@@ -3,6 +3,7 @@ against a model of the cache as plain lists of values, and the refusals of
 the C entry points and of the tensor wrappers, none of which reaches a GPU."""
 import ctypes as C
 import random
+import struct
 
 import pytest
 import torch
@@ -131,6 +132,8 @@ def test_allocator_refusals():
             paged.PageAllocator(*bad)
 
 
+# r4q_paged_cache in the platform's C layout
+PAGED_CACHE = struct.Struct("@PPlliiiPliiPP")
 P16 = C.c_void_p(256)                             # never dereferenced: validation fails first
 
 
@@ -138,7 +141,7 @@ def cache(**kw):
     d = dict(k_pages=256, v_pages=256, k_stride=0, v_stride=0, n_pages=4, page=16, Hk=2, table=256, ld_table=4, seqs=3,
              max_blocks=4, k_scale=0, v_scale=0)
     d.update({k: v or 0 for k, v in kw.items()})
-    return L.PAGED_CACHE.pack(*d.values())
+    return PAGED_CACHE.pack(*d.values())
 
 
 def attn(c=None, q=P16, ldq=512, seq=P16, o=P16, ldo=512, B=2, H=4, flags=0, ws=P16, ws_bytes=1 << 40):
