@@ -4,7 +4,7 @@
 //   o = sum_j p_j V_j / sum_j p_j,   p_j = 2^(s_j - m),   s_j = q.K_j ks log2(e) / sqrt(128)
 //
 // in one pass over K and V with the running maximum m; parts of a sequence join
-// as (m, l, O): M = max m, weights 2^(m - M).
+// as (m, l, O): M = max m, weights 2^(m - M), any m that l and O were taken from.
 //
 // Bound: HBM, 256 bytes per position and kv head; the arithmetic (tensor cores
 // through m16n8k16, FP8 -> f16 by the hardware pair conversion) has to hide
@@ -315,7 +315,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     look_up(beg);
     uint32_t qa[8], qb[8];
-    float m = kLowest, l = 0.f, scale = 0.f, oacc[16][4];
+    // the maximum, and what scores are taken from: m - 15, or m itself where fp32 cannot tell them apart
+    float m = kLowest, base = kLowest, l = 0.f, scale = 0.f, oacc[16][4];
     int seq = 0;
     bool first = at.t == 0;                                   // the segment began in this warp
     auto start_segment = [&]() {
@@ -329,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint4 v = head < a.Hg ? qp[i] : make_uint4(0, 0, 0, 0);
         qa[2 * i] = v.x; qb[2 * i] = v.y; qa[2 * i + 1] = v.z; qb[2 * i + 1] = v.w;
       }
-      m = kLowest;
+      m = base = kLowest;
       l = 0.f;
 #pragma unroll
       for (int j = 0; j < 16; ++j)
@@ -383,8 +384,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       if (__any_sync(0xffffffffu, mx > m)) {
-        const float mn = fmaxf(m, mx), f = ex2(m - mn);
-        m = mn;
+        m = fmaxf(m, mx);
+        float to = m - kWeightBits;
+        to = m - to > kWeightBits ? m : to;                   // from 2^24 on m - 15 may round to m - 16: 2^16 is no f16
+        const float f = ex2(base - to);
+        base = to;
         l *= f;
 #pragma unroll
         for (int j = 0; j < 16; ++j)
@@ -392,7 +396,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 4; ++i) oacc[j][i] *= f;
       }
       uint32_t ph[4], pl[4];                                  // rounded weights and remainders
-      const float base = m - kWeightBits;
 #pragma unroll
       for (int nt = 0; nt < 4; ++nt) {
         const float e0 = ex2(sc[nt][0] - base), e1 = ex2(sc[nt][1] - base);
@@ -452,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                           oacc[j + 3][1] + oacc[j + 3][3]);
         }
         if (t == 0) {
-          p[kHeadDim] = m;
+          p[kHeadDim] = base;
           p[kHeadDim + 1] = l;
         }
         if (first && last) {

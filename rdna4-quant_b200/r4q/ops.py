@@ -452,7 +452,8 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     ``k_out`` if given.  ``k_scale`` / ``v_scale``: fp32 [Hk], stored byte =
     enc(x / scale), the bytes of the contiguous cache; ``full_range`` keeps
     256 .. 448 apart, which its codec stores as 448.  Rows, positions and page
-    ids out of range write nothing and are reported by ``check_status``."""
+    ids out of range write nothing and are reported by ``check_status``; two
+    tokens must not name one position."""
     return _checked(_native.paged_kv_write(k, v, k_pages, v_pages, block_table, positions, rows, q, q_w, k_w, cos, sin,
                                            q_out, k_out, k_scale, v_scale, eps, L.KV_FULL_RANGE if full_range else 0),
                     "r4q_paged_kv_write")

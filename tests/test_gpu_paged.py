@@ -171,6 +171,24 @@ def test_attention_scores_of_any_finite_size():
         assert ((o[0].double() - mean.mean(0)).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("top", [t << e for e in range(21, 27) for t in (9, 13, 15)])
+def test_attention_scores_whose_steps_exceed_one(top):
+    """Half the scores at about `top` (1.9e7 .. 1.0e9, where fp32 steps are 2 .. 64), half at 1 / 8 of it: the mean of V
+    over the first half, which takes every position's weight to be equal and no larger than fp16 holds."""
+    from r4q import ops
+    n = 96
+    kp, vp, table, _, _ = make_paged([n], 1, 16, seed=13)
+    ids = table[0, :n // 16].long()
+    kp[ids] = 0x28                                    # 0.25 = 2 / 8
+    kp[ids[::2]] = 0x40                               # 2.0
+    mean = decode_lut()[vp[ids[::2], 0].reshape(-1, D).long()]
+    q = (1 + torch.arange(8, device="cuda") / 64)[None, :, None].expand(1, 8, D).half()
+    scale = torch.tensor([top / (2 * D / D ** 0.5 * 1.4426950408889634)], device="cuda")
+    o = ops.paged_flash_decode(q, kp, vp, table, torch.tensor([n], device="cuda"), k_scale=scale)
+    tol = mean.abs().mean(0) * (2.0 ** -20 + (64 + n / 8) * U) + mean.mean(0).abs() * 2.0 ** -11 + 2.0 ** -25
+    assert ((o[0].double() - mean.mean(0)).abs() <= tol).all()
+
+
 def test_attention_views_strides_and_shared_pages():
     """q out of a wider row, K and V interleaved in one pool, a table with wider rows and more of them than the
     batch, an output with its own stride; two sequences on the same pages give the same result."""
