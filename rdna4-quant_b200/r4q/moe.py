@@ -83,7 +83,7 @@ class MoEDecoder:
     and V go to the pages of sequences 0 .. batch - 1 instead of the model's
     contiguous caches, and every row has its own position: sequences of
     different lengths, forks that share a prefix, idle rows.  Positions a step
-    writes must have been reserved (``pages.extend``)."""
+    writes must have been reserved (``pages.extend``), on pages of the row's own."""
 
     def __init__(self, model: dict, cfg: dict, batch: int = 1, comm=None, pages=None):
         self.m, self.cfg, self.B = model, cfg, batch
@@ -197,6 +197,8 @@ class MoEDecoder:
                 if not -1 <= p < self.pages.lengths[b] or p >= self.m['rope_cos'].shape[0]:
                     raise ValueError(f"row {b}: position {p} outside the {self.pages.lengths[b]} reserved ones or "
                                      f"the {self.m['rope_cos'].shape[0]} rows of the RoPE tables")
+                if p >= 0:
+                    self.pages.alloc.check_writable(b, p + 1, p)
         self.h_in.copy_(hidden.reshape(self.B, -1))
         if self.pages is None:
             self.seq.fill_(pos + 1)

@@ -119,11 +119,11 @@ class PageAllocator:
             self.lengths[s] = end
         return plan
 
-    def check_writable(self, seq: int, end: int) -> None:
-        """ValueError unless the sequence holds positions [0, end) on pages that no other one shares."""
+    def check_writable(self, seq: int, end: int, start: int = 0) -> None:
+        """ValueError unless the sequence holds positions [start, end) on pages that no other one shares."""
         if self.lengths[self._seq(seq)] < end:
             raise ValueError(f"sequence {seq} holds {self.lengths[seq]} positions, not {end}")
-        shared = [p for p in self.blocks[seq][:-(-end // self.page)] if self.refs[p] > 1]
+        shared = [p for p in self.blocks[seq][start // self.page:-(-end // self.page)] if self.refs[p] > 1]
         if shared:
             raise ValueError(f"sequence {seq} shares pages {shared[:4]} with another one")
 

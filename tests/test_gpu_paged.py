@@ -697,6 +697,26 @@ def test_moe_decoder_on_pages_forks_idles_and_compacts():
     ops.check_status()
 
 
+def test_moe_decoder_refuses_pages_that_another_sequence_shares():
+    """A fork without an extend: a step at a position on a shared page would change what the other sequence reads."""
+    from r4q import moe, paged
+    m = moe.build_moe_model(CFG, dev(), seed=3, max_seq=64, batch=2)
+    pages = paged.PagedKVCache(2, 8, 2, 16, 2, 4, dev())
+    dec = moe.MoEDecoder(m, CFG, batch=2, pages=pages)
+    x = m['embed'][:2].clone()
+    pages.extend({0: 1})
+    dec.step(x, [0, -1])
+    pages.fork(0, 1)
+    before = pages.pool.clone()
+    for pos in ([0, -1], [-1, 0], [0, 0]):
+        with pytest.raises(ValueError):
+            dec.step(x, pos)
+    assert torch.equal(pages.pool, before)
+    pages.extend({1: 1})
+    dec.step(x, [-1, 1])
+    dec.step(x, [0, 1])
+
+
 def test_prefill_into_pages_then_decode_attention():
     """prefill_logits into pages: the logits of a prefill into the contiguous cache (5e-3, the prefill's tolerance),
     and cache codes that differ by a step at most: the paged write encodes K unrounded, the other one from fp16."""

@@ -109,6 +109,19 @@ def test_check_writable():
     a.check_writable(1, 20)
 
 
+def test_check_writable_from_a_position():
+    a = paged.PageAllocator(8, 16, 2, 4)
+    a.extend({0: 40})
+    a.fork(0, 1, 20)                              # pages 0 and 1 are shared, 2 is not
+    a.check_writable(0, 40, 39)
+    a.check_writable(0, 33, 32)
+    for end, start in ((32, 31), (33, 31), (1, 0), (41, 40)):
+        with pytest.raises(ValueError):
+            a.check_writable(0, end, start)
+    a.extend({1: 1})
+    a.check_writable(1, 21, 20)
+
+
 def test_allocator_refusals():
     a = paged.PageAllocator(4, 16, 3, 2)
     a.extend({0: 20})
