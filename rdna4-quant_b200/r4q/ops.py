@@ -439,7 +439,7 @@ def _checked(r, name: str):
 def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                    block_table: torch.Tensor, positions: torch.Tensor, *, rows: Optional[torch.Tensor] = None,
                    q: Optional[torch.Tensor] = None, q_w=None, k_w=None, cos=None, sin=None, q_out=None, k_out=None,
-                   k_scale=None, v_scale=None, eps: float = 1e-6, full_range: bool = False) -> Optional[torch.Tensor]:
+                   k_scale=None, v_scale=None, eps: float = 1e-6, full_range: bool = True) -> Optional[torch.Tensor]:
     """New tokens into the pages of a paged FP8 cache (r4q_paged_kv_write).
 
     k, v fp16 [M, Hk, 128] (views of a wider row are fine); pages uint8
@@ -450,10 +450,11 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pa
     position first; q [M, H, 128] then comes back in ``q_out`` (default: a new
     tensor, undefined in the rows of padding; q itself for in place) and k in
     ``k_out`` if given.  ``k_scale`` / ``v_scale``: fp32 [Hk], stored byte =
-    enc(x / scale), the bytes of the contiguous cache; ``full_range`` keeps
-    256 .. 448 apart, which its codec stores as 448.  Rows, positions and page
-    ids out of range write nothing and are reported by ``check_status``; two
-    tokens must not name one position."""
+    enc(x / scale) with E4M3's whole range: three mantissa bits, ties away from
+    zero, zero below 2^-6, at most 448.  ``full_range=False`` takes the
+    contiguous cache's codec instead, which stores 448 from 248 on.  Rows,
+    positions and page ids out of range write nothing and are reported by
+    ``check_status``; two tokens must not name one position."""
     return _checked(_native.paged_kv_write(k, v, k_pages, v_pages, block_table, positions, rows, q, q_w, k_w, cos, sin,
                                            q_out, k_out, k_scale, v_scale, eps, L.KV_FULL_RANGE if full_range else 0),
                     "r4q_paged_kv_write")

@@ -183,11 +183,12 @@ class PagedKVCache:
     current stream, like any kernel: use the cache on that stream, or make
     another one wait for it.  Tensors keep their addresses, so captured
     graphs that read them stay valid across operations.  ``k_scales`` /
-    ``v_scales``: per layer fp32 [Hk]; ``full_range``: see ops.paged_kv_write."""
+    ``v_scales``: per layer fp32 [Hk]; ``full_range``: False stores values from
+    248 on as the contiguous cache does (ops.paged_kv_write)."""
 
     def __init__(self, layers: int, n_pages: int, kv_heads: int, page: int, seqs: int, max_blocks: int, device,
                  k_scales: Optional[Sequence[torch.Tensor]] = None, v_scales: Optional[Sequence[torch.Tensor]] = None,
-                 full_range: bool = False):
+                 full_range: bool = True):
         self.alloc = PageAllocator(n_pages, page, seqs, max_blocks)
         self.layers, self.page = int(layers), int(page)
         self.pool = torch.zeros(layers, 2, n_pages, kv_heads, page, 128, dtype=torch.uint8, device=device)
