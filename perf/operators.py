@@ -299,7 +299,7 @@ def run(state):
     if op == "write":
         norm = dict(q=s["q"], q_w=s["qw"], k_w=s["kw"], cos=s["cos"], sin=s["sin"]) if s["case"]["norm"] else {}
         q = ops.paged_kv_write(s["k"], s["v"], s["kp"], s["vp"], s["table"], s["pos"], rows=s["rows"],
-                               k_scale=s["scale"], v_scale=s["scale"], full_range=True, **norm)
+                               k_scale=s["scale"], v_scale=s["scale"], **norm)
         out = {"k": s["kp"].view(F8), "v": s["vp"].view(F8)}
         return dict(out, q=q) if s["case"]["norm"] else out
     if op == "attn":
