@@ -224,7 +224,13 @@ class BatchedEngine:
                 self.pos[s] = len(r.prompt)
                 tok = sample(lg, r.temperature, r.top_p, self._gen(r))
                 if r.logprobs is not None:
-                    r.token_logprobs += self.be.logprobs(lg.reshape(1, -1), [tok], r.logprobs)
+                    try:
+                        r.token_logprobs += self.be.logprobs(lg.reshape(1, -1), [tok], r.logprobs)
+                    except BaseException:  # no token yet: it waits again, with its first draw before it
+                        self.slots[s], self.pos[s] = None, 0
+                        self.gens.pop(r.id, None)
+                        self.queue.insert(0, r)
+                        raise
                 self._emit(s, r, tok)
 
     @property
@@ -243,20 +249,31 @@ class BatchedEngine:
             if greedy:
                 am = torch.argmax(logits[greedy], dim=-1).tolist()
             picks = dict(zip(greedy, am)) if greedy else {}
-            for s in rows:
-                r = self.slots[s]
-                if s not in picks:
-                    picks[s] = sample(logits[s], r.temperature, r.top_p, self._gen(r))
             wanted = [s for s in rows if self.slots[s].logprobs is not None]
-            if wanted:                     # one call for the rows that want them, with the largest k
-                lps = self.be.logprobs(logits if len(wanted) == self.batch else logits[wanted],
-                                       [picks[s] for s in wanted], max(self.slots[s].logprobs for s in wanted))
-                for s, lp in zip(wanted, lps):
+            lps, undo = {}, {}             # generators of draws not emitted yet, as they were before
+            try:
+                if wanted:                 # one call for the rows that want them, with the largest k: they draw ahead
+                    for s in wanted:
+                        if s not in picks:
+                            r = self.slots[s]
+                            gen = self._gen(r)
+                            undo[s] = gen, gen.get_state()
+                            picks[s] = sample(logits[s], r.temperature, r.top_p, gen)
+                    lps = dict(zip(wanted, self.be.logprobs(
+                        logits if len(wanted) == self.batch else logits[wanted], [picks[s] for s in wanted],
+                        max(self.slots[s].logprobs for s in wanted))))
+                for s in rows:
                     r = self.slots[s]
-                    r.token_logprobs.append(replace(lp, top=lp.top[:r.logprobs]))
-            for s in rows:
-                self.pos[s] += 1
-                self._emit(s, self.slots[s], picks[s])
+                    if s not in picks:
+                        picks[s] = sample(logits[s], r.temperature, r.top_p, self._gen(r))
+                    undo.pop(s, None)
+                    if s in lps:
+                        r.token_logprobs.append(replace(lps[s], top=lps[s].top[:r.logprobs]))
+                    self.pos[s] += 1
+                    self._emit(s, r, picks[s])
+            finally:                       # a callback raised: the rows behind it are decoded again
+                for gen, state in undo.values():
+                    gen.set_state(state)
             self.steps += 1
             return len(rows)
 
