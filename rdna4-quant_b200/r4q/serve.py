@@ -260,7 +260,7 @@ class BatchedEngine:
                             undo[s] = gen, gen.get_state()
                             picks[s] = sample(logits[s], r.temperature, r.top_p, gen)
                     lps = dict(zip(wanted, self.be.logprobs(
-                        logits if len(wanted) == self.batch else logits[wanted], [picks[s] for s in wanted],
+                        logits if len(wanted) == logits.shape[0] else logits[wanted], [picks[s] for s in wanted],
                         max(self.slots[s].logprobs for s in wanted))))
                 for s in rows:
                     r = self.slots[s]

@@ -91,3 +91,17 @@ def test_a_step_without_likelihoods_is_repeated_as_it_was(fail_at):
     for r, kw in ((ra, a), (rb, b)):
         want = alone(kw)
         assert r.tokens == want.tokens and r.token_logprobs == want.token_logprobs
+
+
+def test_backend_with_more_rows_than_the_engine_has_slots():
+    """Its logits carry rows of no request: they are not handed to the likelihoods."""
+    class Wide(Backend):
+        def step(self, tokens, positions):
+            return torch.cat([super().step(tokens, positions), torch.zeros(2, V)])
+
+        def logprobs(self, logits, tokens, k):
+            assert logits.shape[0] == len(tokens)
+            return super().logprobs(logits, tokens, k)
+    r, = serve.BatchedEngine(Wide(), batch=1).generate([[1]], max_new_tokens=4, logprobs=2)
+    want = alone(dict(A, logprobs=2))
+    assert r.tokens == want.tokens and r.token_logprobs == want.token_logprobs
