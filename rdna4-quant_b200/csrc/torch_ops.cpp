@@ -102,8 +102,8 @@ struct Cache {
     const int64_t P = k.size(0), Hk = k.size(1), page = k.size(2);
     for (const Tensor* t : {&k, &v})
       TORCH_CHECK_VALUE(t->stride(3) == 1 && (page == 1 || t->stride(2) == 128) &&
-                            (Hk == 1 || t->stride(1) == page * 128),
-                        "each page must be contiguous [kv heads, page, 128]");
+                            (Hk == 1 || t->stride(1) == page * 128) && (P <= 1 || t->stride(0) >= Hk * page * 128),
+                        "each page must be contiguous [kv heads, page, 128] and lie behind the one before");
     TORCH_CHECK_TYPE(table.scalar_type() == at::kInt && table.dim() == 2,
                      "block_table must be int32 [sequences, blocks]");
     const int64_t S = table.size(0), nb = table.size(1);
@@ -194,8 +194,8 @@ PyObject* paged_kv_write(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const double eps = PyFloat_AsDouble(a[16]);
   if (eps == -1.0 && PyErr_Occurred()) throw python_error();
   int flags = (int)PyLong_AsLong(a[17]);
-  const Gpu gpu(k_, v_, kp, vp, table, pos, rows, q_, q_w, k_w, cos, sin, q_out_, k_out_, ks, vs);
   const Cache cache(kp, vp, table, ks, vs);
+  const Gpu gpu(k_, v_, kp, vp, table, pos, rows, q_, q_w, k_w, cos, sin, q_out_, k_out_, ks, vs);
   const Heads k(k_, "k", -1, cache.c.Hk, false), v(v_, "v", k.rows, cache.c.Hk, false);
   pos = vector(pos, "positions", at::kLong, k.rows);
   if (rows.defined()) rows = vector(rows, "rows", at::kInt, k.rows);
@@ -245,9 +245,9 @@ PyObject* paged_flash_decode(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   Tensor seq = tensor(a[4], "seq_lens");
   const Tensor ks = optional(a[5], "k_scale"), vs = optional(a[6], "v_scale"), out_ = optional(a[8], "out");
   const int flags = (int)PyLong_AsLong(a[7]);
+  const Cache cache(kp, vp, table, ks, vs);
   const Gpu gpu(q_, kp, vp, table, seq, ks, vs, out_);
   const Heads q(q_, "q", -1, -1, false);
-  const Cache cache(kp, vp, table, ks, vs);
   seq = vector(seq, "seq_lens", at::kLong, q.rows);
   const Heads out(out_.defined() ? out_ : at::empty({q.rows, q.heads, 128}, q_.options()), "out", q.rows, q.heads, true);
   const int B = int_size(q.rows, "sequences"), H = int_size(q.heads, "heads");
