@@ -1,6 +1,7 @@
 // Paged FP8 KV cache: new tokens into pages (with the per-head RMSNorm + RoPE
 // of q and k), page copies over all layers, block-table updates, and the
 // status of the kernels that keep their status words in the library.
+#include <algorithm>
 #include <cstdlib>
 #include <cstring>
 
@@ -355,6 +356,17 @@ extern "C" int r4q_kv_table_set(int* table, long ld, int rows, int cols, const i
     if (r[i] < 0 || r[i] >= rows || c[i] < 0 || c[i] >= cols)
       return set_error(R4Q_ERR_ARG, "kv_table_set: cell %d (%d, %d) outside the table of %d x %d", i, r[i], c[i], rows,
                        cols);
+  if (n > 1) {                                       // threads write in any order: a cell twice has no one value
+    long* cell = (long*)malloc(n * sizeof(long));
+    if (!cell) return set_error(R4Q_ERR_CAPACITY, "kv_table_set: no host memory for %d cells", n);
+    for (int i = 0; i < n; ++i) cell[i] = (long)r[i] * cols + c[i];
+    std::sort(cell, cell + n);
+    const long* twice = std::adjacent_find(cell, cell + n);
+    const long bad = twice == cell + n ? -1 : *twice;
+    free(cell);
+    if (bad >= 0)
+      return set_error(R4Q_ERR_ARG, "kv_table_set: cell (%ld, %ld) is written twice", bad / cols, bad % cols);
+  }
   for (int at = 0; at < n; at += kMaxCells) {
     const int part = n - at < kMaxCells ? n - at : kMaxCells;
     Cells cells;

@@ -30,3 +30,18 @@ def test_layouts_that_are_pages_pass_on_to_the_device_check():
             ops.paged_flash_decode(K, kp, vp, TABLE, POS)
         with pytest.raises(ValueError, match="CUDA"):
             ops.paged_kv_write(K, K, kp, vp, TABLE, POS)
+
+
+def test_a_table_cell_twice_is_refused():
+    """The kernel writes the cells in any order."""
+    import ctypes as C
+    import random
+    from r4q import lib as L
+
+    def put(cells):
+        r, c = ((C.c_int * len(cells))(*x) for x in zip(*cells))
+        return L.LIB.r4q_kv_table_set(C.c_void_p(256), 50, 60, 50, r, c, r, len(cells), None)   # refused before any launch
+    many = [(i, j) for i in range(60) for j in range(50)]
+    random.Random(1).shuffle(many)
+    for cells in ([(0, 0), (0, 0)], [(1, 2), (2, 1), (1, 2)], many + [many[7]]):
+        assert put(cells) == -1 and "twice" in L.last_error()
