@@ -145,10 +145,12 @@ std::vector<int> host_ints(PyObject* o, const char* name) {
   }
   THPObjectPtr seq(PySequence_Fast(o, name));
   if (!seq) throw python_error();
-  const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq.get());
-  out.reserve(n);
-  for (Py_ssize_t i = 0; i < n; ++i) {
-    const long long v = PyLong_AsLongLong(PySequence_Fast_GET_ITEM(seq.get(), i));
+  out.reserve(PySequence_Fast_GET_SIZE(seq.get()));
+  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq.get()); ++i) {     // an item's __index__ may change the list
+    PyObject* item = PySequence_Fast_GET_ITEM(seq.get(), i);
+    Py_INCREF(item);
+    const THPObjectPtr held(item);
+    const long long v = PyLong_AsLongLong(item);
     if (v == -1 && PyErr_Occurred()) {
       if (!PyErr_ExceptionMatches(PyExc_OverflowError)) throw python_error();
       PyErr_Clear();
