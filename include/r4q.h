@@ -282,12 +282,15 @@ size_t r4q_paged_flash_decode_workspace_bytes(int B, int H, int Hk, int page, in
 int r4q_paged_flash_decode(const void* q, long ldq, const r4q_paged_cache* cache, const long long* seq_lens, void* o,
                            long ldo, int B, int H, int flags, void* workspace, size_t ws_bytes, void* stream);
 
-/* R4Q_ERR_PAGE if a paged kernel of the current device met an id out of range
- * since the last clear, R4Q_ERR_TIMEOUT if a bounded wait of the paged attention
- * or of r4q_token_logprobs gave up (those outputs are not valid), else R4Q_OK.
+/* R4Q_ERR_TIMEOUT if a bounded wait of the paged attention or of
+ * r4q_token_logprobs on the current device gave up since the last clear (those
+ * outputs are not valid), else R4Q_ERR_PAGE if a paged kernel met an id out of
+ * range, else R4Q_OK; the message names everything that was met.
  * Their status words live in the library, one per device: no workspace to pass.
  * Synchronises the device. */
 int r4q_kernel_status(int clear);
+/* Test hook: what r4q_kernel_status says of status words (1: a wait gave up, 2: an id out of range). */
+int r4q_debug_status_of(int write, int attention, int likelihoods);
 
 /* pool[l][dst[i]] = pool[l][src[i]] for every i < n and every l < outer: pages of
  * page_bytes, page_stride apart, in `outer` pools (layers, K and V)

@@ -2,6 +2,7 @@
 // of q and k), page copies over all layers, block-table updates, and the
 // status of the kernels that keep their status words in the library.
 #include <algorithm>
+#include <cstdio>
 #include <cstdlib>
 #include <cstring>
 
@@ -225,6 +226,22 @@ __global__ void table_set_kernel(int* table, long ld, int n, const __grid_consta
 
 }  // namespace
 
+// What the status words say.  A wait that gave up voids a whole call's outputs, a bad
+// page those of its row: the first gives the code, and the message names both.
+static int status_of(int write, int attn, int likelihood) {
+  const bool aw = attn & kPagedTimeout, lw = likelihood & kPagedTimeout;
+  const bool wp = write & kPagedBadPage, ap = attn & kPagedBadPage;
+  char wait[160] = "", page[160] = "";
+  if (aw || lw)
+    snprintf(wait, sizeof(wait), "a bounded wait of %s%s%s gave up since the last check: those outputs are not valid",
+             aw ? "the paged attention" : "", aw && lw ? " and " : "", lw ? "the likelihood kernel" : "");
+  if (wp || ap)
+    snprintf(page, sizeof(page), "%s%s%s met a row, position, length or page id outside the cache since the last check",
+             wp ? "a paged write" : "", wp && ap ? " and " : "", ap ? "a paged attention" : "");
+  if (!*wait && !*page) return R4Q_OK;
+  return set_error(*wait ? R4Q_ERR_TIMEOUT : R4Q_ERR_PAGE, "%s%s%s", wait, *wait && *page ? "; " : "", page);
+}
+
 int paged_view(const char* what, const r4q_paged_cache* c, PagedView* out) {
   if (!c || !c->k_pages || !c->v_pages || !c->table) return set_error(R4Q_ERR_ARG, "%s: null cache pointer", what);
   if (c->page < 16 || c->page % 16 || c->page > 4096)
@@ -394,11 +411,9 @@ extern "C" int r4q_kernel_status(int clear) {
     cudaGetLastError();
     return set_error(R4Q_ERR_CUDA, "kernel_status: %s", cudaGetErrorString(e));
   }
-  if ((a | b) & kPagedBadPage)
-    return set_error(R4Q_ERR_PAGE, "a paged %s met a row, position, length or page id outside the cache since the last "
-                     "check", a & kPagedBadPage ? "write" : "attention");
-  if ((b | c) & kPagedTimeout)
-    return set_error(R4Q_ERR_TIMEOUT, "a bounded wait of the %s kernel gave up since the last check: its outputs are "
-                     "not valid", b & kPagedTimeout ? "paged attention" : "likelihood");
-  return R4Q_OK;
+  return status_of(a, b, c);
+}
+
+extern "C" int r4q_debug_status_of(int write, int attention, int likelihoods) {
+  return status_of(write, attention, likelihoods);
 }
