@@ -759,12 +759,7 @@ int launch(const void* logits, long ld, const long long* tokens, int M, int V, i
 
 }  // namespace
 
-cudaError_t logprob_status(int clear, int* word) {
-  const int zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(word, g_logprob_status, sizeof(int));
-  if (e == cudaSuccess && *word && clear) e = cudaMemcpyToSymbol(g_logprob_status, &zero, sizeof(int));
-  return e;
-}
+cudaError_t logprob_status_word(int** word) { return cudaGetSymbolAddress((void**)word, g_logprob_status); }
 
 }  // namespace r4q
 

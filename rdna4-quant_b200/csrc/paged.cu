@@ -5,6 +5,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <mutex>
 
 #include "f32x2.cuh"
 #include "paged.cuh"
@@ -226,6 +227,14 @@ __global__ void table_set_kernel(int* table, long ld, int n, const __grid_consta
 
 }  // namespace
 
+// The status words as they are, cleared in the same step: what a kernel that another
+// thread launches meanwhile sets is either taken here or left for the next call.
+static __device__ int g_taken[3];
+static __global__ void take_status_kernel(int* write, int* attn, int* likelihood, int clear) {
+  int* const word[3] = {write, attn, likelihood};
+  for (int i = 0; i < 3; ++i) g_taken[i] = clear ? atomicExch(word[i], 0) : atomicOr(word[i], 0);
+}
+
 // What the status words say.  A wait that gave up voids a whole call's outputs, a bad
 // page those of its row: the first gives the code, and the message names both.
 static int status_of(int write, int attn, int likelihood) {
@@ -400,18 +409,23 @@ extern "C" int r4q_kv_table_set(int* table, long ld, int rows, int cols, const i
 }
 
 extern "C" int r4q_kernel_status(int clear) {
-  int a = 0, b = 0, c = 0;
-  const int zero = 0;
+  static std::mutex mu;                              // g_taken is one per device
+  std::lock_guard<std::mutex> lk(mu);
+  int *write = nullptr, *attn = nullptr, *likelihood = nullptr, word[3] = {0, 0, 0};
   cudaError_t e = cudaDeviceSynchronize();
-  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&a, g_write_status, sizeof(int));
-  if (e == cudaSuccess && a && clear) e = cudaMemcpyToSymbol(g_write_status, &zero, sizeof(int));
-  if (e == cudaSuccess) e = paged_attn_status(clear, &b);
-  if (e == cudaSuccess) e = logprob_status(clear, &c);
+  if (e == cudaSuccess) e = cudaGetSymbolAddress((void**)&write, g_write_status);
+  if (e == cudaSuccess) e = paged_attn_status_word(&attn);
+  if (e == cudaSuccess) e = logprob_status_word(&likelihood);
+  if (e == cudaSuccess) {
+    take_status_kernel<<<1, 1>>>(write, attn, likelihood, clear);
+    e = cudaGetLastError();
+  }
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(word, g_taken, sizeof(word));
   if (e != cudaSuccess) {
     cudaGetLastError();
     return set_error(R4Q_ERR_CUDA, "kernel_status: %s", cudaGetErrorString(e));
   }
-  return status_of(a, b, c);
+  return status_of(word[0], word[1], word[2]);
 }
 
 extern "C" int r4q_debug_status_of(int write, int attention, int likelihoods) {

@@ -37,8 +37,8 @@ struct PagedView {
 
 // Checks the caller's description and fills the view; `what` names the caller.
 int paged_view(const char* what, const r4q_paged_cache* c, PagedView* out);
-// Status words of the attention and the likelihood kernels (the device is idle).
-cudaError_t paged_attn_status(int clear, int* word);
-cudaError_t logprob_status(int clear, int* word);
+// Where the attention's and the likelihood kernels' status words lie on the current device.
+cudaError_t paged_attn_status_word(int** word);
+cudaError_t logprob_status_word(int** word);
 
 }  // namespace r4q

@@ -577,12 +577,7 @@ size_t header_bytes(int B) { return ((size_t)(B + 2) * 4 + 15) / 16 * 16; }
 
 }  // namespace
 
-cudaError_t paged_attn_status(int clear, int* word) {
-  const int zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(word, g_attn_status, sizeof(int));
-  if (e == cudaSuccess && *word && clear) e = cudaMemcpyToSymbol(g_attn_status, &zero, sizeof(int));
-  return e;
-}
+cudaError_t paged_attn_status_word(int** word) { return cudaGetSymbolAddress((void**)word, g_attn_status); }
 
 }  // namespace r4q
 
