@@ -287,7 +287,7 @@ int r4q_paged_flash_decode(const void* q, long ldq, const r4q_paged_cache* cache
  * outputs are not valid), else R4Q_ERR_PAGE if a paged kernel met an id out of
  * range, else R4Q_OK; the message names everything that was met.
  * Their status words live in the library, one per device: no workspace to pass.
- * Synchronises the device, unless none of these kernels has run on it. */
+ * Synchronises the device. */
 int r4q_kernel_status(int clear);
 /* Test hook: what r4q_kernel_status says of status words (1: a wait gave up, 2: an id out of range). */
 int r4q_debug_status_of(int write, int attention, int likelihoods);

@@ -778,7 +778,6 @@ extern "C" int r4q_token_logprobs(const void* logits, int type, long ld, const l
     return set_error(R4Q_ERR_ARG, "token_logprobs: null logits or row stride %ld < %d", ld, V);
   if (!tokens && (logprob || rank)) return set_error(R4Q_ERR_ARG, "token_logprobs: logprob and rank need tokens");
   if (!aligned(logits, type == R4Q_T_F32 ? 4 : 2)) return set_error(R4Q_ERR_ALIGN, "token_logprobs: logits misaligned");
-  paged_or_logprob_runs();
   const auto go = type == R4Q_T_F16 ? launch<__half> : type == R4Q_T_BF16 ? launch<__nv_bfloat16> : launch<float>;
   return go(logits, ld, tokens, M, V, k, logprob, rank, entropy, top_ids, top_logprobs, (cudaStream_t)stream);
 }

@@ -2,7 +2,6 @@
 // of q and k), page copies over all layers, block-table updates, and the
 // status of the kernels that keep their status words in the library.
 #include <algorithm>
-#include <atomic>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -228,16 +227,6 @@ __global__ void table_set_kernel(int* table, long ld, int n, const __grid_consta
 
 }  // namespace
 
-// Whether kernels with these status words were launched on a device: a program that
-// uses none of them is not made to wait for the device by a check.
-constexpr int kMaxDevices = 64;
-static std::atomic<bool> g_ran[kMaxDevices];
-void paged_or_logprob_runs() {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < kMaxDevices && !g_ran[dev].load(std::memory_order_relaxed)) g_ran[dev].store(true);
-}
-
 // The status words as they are, cleared in the same step: what a kernel that another
 // thread launches meanwhile sets is either taken here or left for the next call.
 static __device__ int g_taken[3];
@@ -330,7 +319,6 @@ extern "C" int r4q_paged_kv_write(const void* q, long ldq, const void* k, long l
   a.by_page = fast_div(a.c.page);
   const long warps = (long)M * a.groups;
   if (warps > 0x7ffffff0L) return set_error(R4Q_ERR_ARG, "paged_kv_write: %d tokens of %d heads are too many", M, H);
-  paged_or_logprob_runs();
   const cudaError_t e =
       launch_pdl(paged_write_kernel, dim3((unsigned)((warps * 32 + kWriteThreads - 1) / kWriteThreads)),
                  dim3(kWriteThreads), 0, (cudaStream_t)stream, a);
@@ -421,9 +409,6 @@ extern "C" int r4q_kv_table_set(int* table, long ld, int rows, int cols, const i
 }
 
 extern "C" int r4q_kernel_status(int clear) {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < kMaxDevices && !g_ran[dev].load()) return R4Q_OK;   // nothing to wait for
   static std::mutex mu;                              // g_taken is one per device
   std::lock_guard<std::mutex> lk(mu);
   int *write = nullptr, *attn = nullptr, *likelihood = nullptr, word[3] = {0, 0, 0};

@@ -37,8 +37,6 @@ struct PagedView {
 
 // Checks the caller's description and fills the view; `what` names the caller.
 int paged_view(const char* what, const r4q_paged_cache* c, PagedView* out);
-// Called before a launch of a kernel that has one of the status words.
-void paged_or_logprob_runs();
 // Where the attention's and the likelihood kernels' status words lie on the current device.
 cudaError_t paged_attn_status_word(int** word);
 cudaError_t logprob_status_word(int** word);

@@ -653,7 +653,6 @@ extern "C" int r4q_paged_flash_decode(const void* q, long ldq, const r4q_paged_c
       if (dev < 64) attr_done[dev] = true;
     }
   }
-  paged_or_logprob_runs();
   cudaStream_t s = (cudaStream_t)stream;
   const unsigned ctas = a.per_seg ? (unsigned)(B * Hc) : (unsigned)num_sms();
   cudaError_t e = launch_pdl(paged_attn_kernel, dim3(ctas), dim3(kThreads), smem_bytes(B), s, tmk, tmv, a);

@@ -73,8 +73,7 @@ def check_status(dev: torch.device | int | None = None, clear: bool = True) -> N
     word of every workspace these wrappers hold for the device, of the
     allocation-free GEMV's static scratch and of the paged kernels, which also
     report a page id, position or row outside the cache (R4Q_ERR_PAGE).
-    Synchronises each stream, and the device if paged or likelihood operators
-    have run on it."""
+    Synchronises the device."""
     if dev is None:
         dev = torch.cuda.current_device()
     idx = dev if isinstance(dev, int) else (dev.index if dev.index is not None else torch.cuda.current_device())
