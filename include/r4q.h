@@ -289,6 +289,10 @@ int r4q_paged_flash_decode(const void* q, long ldq, const r4q_paged_cache* cache
  * Their status words live in the library, one per device: no workspace to pass.
  * Synchronises the device. */
 int r4q_kernel_status(int clear);
+/* Test hook: polls before a wait of the paged attention and of r4q_token_logprobs
+ * gives up (default 2^22, the most; negative restores it; 0: at once).  Returns the
+ * previous limit.  A kernel that gave up still waits for its copies in flight. */
+long r4q_debug_wait_limit(long polls);
 /* Test hook: what r4q_kernel_status says of status words (1: a wait gave up, 2: an id out of range). */
 int r4q_debug_status_of(int write, int attention, int likelihoods);
 

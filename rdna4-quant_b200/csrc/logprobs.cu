@@ -57,7 +57,6 @@ constexpr int kMaxCluster = 8;
 constexpr int kUnroll = 4;                // 16-byte words of a lane in a chunk
 constexpr int kChunk = 32 * kUnroll;      // words of a warp's chunk, 2 KB
 constexpr int kStages = 2;                // chunks of a warp's ring
-constexpr int kPolls = 1 << 22;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kTiny = -150.f;           // 2^kTiny is 0 in fp32: also stands for log2 0, where 0 * -inf would be NaN
 
@@ -305,16 +304,6 @@ __device__ __forceinline__ uint64_t merge(uint64_t a, uint64_t b, int lane) {
 
 __device__ int g_logprob_status;         // a bounded wait gave up
 
-__device__ __forceinline__ bool wait_full(uint64_t* bar, unsigned parity) {
-  const uint32_t b = smem_u32(bar);
-  for (int i = 0; i < kPolls; ++i) {
-    uint32_t ok;
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-                 " selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(b), "r"(parity) : "memory");
-    if (ok) return true;
-  }
-  return false;
-}
 __device__ __forceinline__ void copy_chunk(void* dst, const void* src, uint64_t* bar) {
   mbar_expect_tx(bar, kChunk * 16);
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -324,7 +313,7 @@ __device__ __forceinline__ void copy_chunk(void* dst, const void* src, uint64_t*
 template <typename X>
 __global__ void __launch_bounds__(kThreads, kResident)
     logprobs_kernel(const X* __restrict__ logits, long ld, const long long* __restrict__ tokens, int V, int k,
-                    float* logprob, long long* rank_out, float* entropy, long long* top_ids, float* top_lp) {
+                    float* logprob, long long* rank_out, float* entropy, long long* top_ids, float* top_lp, int polls) {
   constexpr int n = Vec<X>::n;
   __shared__ Shared sh;
   extern __shared__ __align__(16) uint4 ring_mem[];    // [warp][stage][kChunk]
@@ -371,11 +360,11 @@ __global__ void __launch_bounds__(kThreads, kResident)
     const int i = base + lane;               // this lane's words: i, i + 32, ..
     uint4* mine = ring + stage * kChunk + lane;
     if (r.bulk(base)) {
-      if (!wait_full(&bars[stage], parity >> stage & 1)) {
+      if (!mbar_wait_warp(&bars[stage], parity >> stage & 1, polls)) {
         // the copies in flight get their time once more; the row's results are void
-        for (int j = 1; j < kStages; ++j) {
+        for (int j = 0; j < kStages; ++j) {
           const int s2 = (stage + j) % kStages, at = base + j * stride;
-          if (at < r.words && r.bulk(at)) wait_full(&bars[s2], parity >> s2 & 1);
+          if (at < r.words && r.bulk(at)) mbar_wait_warp(&bars[s2], parity >> s2 & 1, kWaitPolls);
         }
         if (lane == 0) atomicOr(&g_logprob_status, kPagedTimeout);
         nan = 1;
@@ -748,7 +737,7 @@ int launch(const void* logits, long ld, const long long* tokens, int M, int V, i
     const cudaError_t e = cudaLaunchKernelEx(
         &cfg, logprobs_kernel<X>, (const X*)logits + o * ld, ld, tokens ? tokens + o : nullptr, V, k,
         logprob ? logprob + o : nullptr, rank ? rank + o : nullptr, entropy ? entropy + o : nullptr,
-        top_ids ? top_ids + o * k : nullptr, top_lp ? top_lp + o * k : nullptr);
+        top_ids ? top_ids + o * k : nullptr, top_lp ? top_lp + o * k : nullptr, wait_polls());
     if (e != cudaSuccess) {
       cudaGetLastError();
       return set_error(R4Q_ERR_CUDA, "logprobs_kernel (cluster %d): %s", C, cudaGetErrorString(e));

@@ -2,6 +2,7 @@
 // of q and k), page copies over all layers, block-table updates, and the
 // status of the kernels that keep their status words in the library.
 #include <algorithm>
+#include <atomic>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -227,6 +228,9 @@ __global__ void table_set_kernel(int* table, long ld, int n, const __grid_consta
 
 }  // namespace
 
+static std::atomic<int> g_wait_polls{kWaitPolls};
+int wait_polls() { return g_wait_polls.load(std::memory_order_relaxed); }
+
 // The status words as they are, cleared in the same step: what a kernel that another
 // thread launches meanwhile sets is either taken here or left for the next call.
 static __device__ int g_taken[3];
@@ -426,6 +430,10 @@ extern "C" int r4q_kernel_status(int clear) {
     return set_error(R4Q_ERR_CUDA, "kernel_status: %s", cudaGetErrorString(e));
   }
   return status_of(word[0], word[1], word[2]);
+}
+
+extern "C" long r4q_debug_wait_limit(long polls) {
+  return g_wait_polls.exchange(polls < 0 || polls > kWaitPolls ? kWaitPolls : (int)polls);
 }
 
 extern "C" int r4q_debug_status_of(int write, int attention, int likelihoods) {

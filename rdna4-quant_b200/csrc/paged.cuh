@@ -9,6 +9,7 @@
 namespace r4q {
 
 constexpr int kHeadDim = 128;
+constexpr int kWaitPolls = 1 << 22;  // of a bounded wait of these kernels, before it gives up
 constexpr int kPagedTimeout = 1;   // a bounded wait gave up
 constexpr int kPagedBadPage = 2;   // a row, position, length or page id outside the cache
 
@@ -37,6 +38,9 @@ struct PagedView {
 
 // Checks the caller's description and fills the view; `what` names the caller.
 int paged_view(const char* what, const r4q_paged_cache* c, PagedView* out);
+// Polls that a launch gives its waits: kWaitPolls, or what r4q_debug_wait_limit set.  The
+// wait for copies still in flight after that always has kWaitPolls.
+int wait_polls();
 // Where the attention's and the likelihood kernels' status words lie on the current device.
 cudaError_t paged_attn_status_word(int** word);
 cudaError_t logprob_status_word(int** word);

@@ -56,7 +56,6 @@ constexpr int kPitch = 132;                       // floats of a part's head: O[
 constexpr int kPartFloats = kGroup * kPitch;
 constexpr int kMaxBatch = 2048;
 constexpr int kJoinWarps = 4;
-constexpr int kWaitPolls = 1 << 22;
 constexpr float kWeightBits = 15.f;               // weights are carried times 2^15
 constexpr float kLowest = -3e38f;                 // a maximum before the first score: no finite score is below it
 
@@ -71,6 +70,7 @@ struct AttnArgs {
   FastDiv by_page, by_Hc, by_chunks, by_ctas;
   int per_seg;       // a CTA per (sequence, head, group) instead of equal runs
   int two_boxes;     // 16-position boxes
+  int polls;         // of the wait for a tile
   int* header;       // workspace: tiles per CTA, then the prefix sums of tiles [B + 1]
   float* parts;      // workspace: [CTA][2][kPartFloats]
 };
@@ -79,16 +79,6 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-__device__ __forceinline__ bool wait_full(uint64_t* bar, unsigned parity) {
-  const uint32_t b = smem_u32(bar);
-  for (int i = 0; i < kWaitPolls; ++i) {
-    uint32_t ok;
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-                 " selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(b), "r"(parity) : "memory");
-    if (ok) return true;
-  }
-  return false;
 }
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int row, int page, uint64_t* bar) {
   asm volatile(
@@ -344,12 +334,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     int slot = 0;
     unsigned parity = 0;
     for (int x = beg; x < end; ++x) {
-      if (!wait_full(&wbars[slot], parity)) {                 // drain what is in flight and stop
+      if (!mbar_wait_warp(&wbars[slot], parity, a.polls)) {   // drain what is in flight and stop
         if (lane == 0) atomicOr(&g_attn_status, kPagedTimeout);
-        for (int y = x + 1; y < min(end, x + kSlots); ++y) {
+        for (int y = x; y < min(end, x + kSlots); ++y) {
+          mbar_wait_warp(&wbars[slot], parity, kWaitPolls);
           slot = slot + 1 == kSlots ? 0 : slot + 1;
           if (slot == 0) parity ^= 1;
-          wait_full(&wbars[slot], parity);
         }
         break;
       }
@@ -628,6 +618,7 @@ extern "C" int r4q_paged_flash_decode(const void* q, long ldq, const r4q_paged_c
   a.o = (__half*)o; a.ldo = ldo;
   a.B = B; a.H = H; a.fwht = (flags & R4Q_ATTN_FWHT) ? 1 : 0;
   a.two_boxes = a.c.page % kTile != 0;
+  a.polls = wait_polls();
   if (need) {
     a.header = (int*)workspace;
     a.parts = (float*)((uint8_t*)workspace + header_bytes(B));

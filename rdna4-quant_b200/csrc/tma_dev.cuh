@@ -63,6 +63,17 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* b, unsigned parity, int* sta
   return false;
 }
 
+// Bounded wait of a whole warp, with one answer for all of it: lanes that gave up while
+// others saw the copy land would leave them alone in the next full-warp operation.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, unsigned parity, int polls) {
+  const uint32_t b = smem_u32(bar);
+  uint32_t ok = 0;
+  for (int i = 0; i < polls && !ok; ++i)
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+                 " selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(b), "r"(parity) : "memory");
+  return __all_sync(0xffffffffu, ok);
+}
+
 // L2 cache policy for data read exactly once (streamed weights).
 __device__ __forceinline__ uint64_t l2_policy_evict_first() {
   uint64_t pol;

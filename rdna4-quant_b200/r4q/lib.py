@@ -96,6 +96,7 @@ _SIGS = {
     "r4q_paged_flash_decode_workspace_bytes": (sz_t, [i32, i32, i32, i32, i32]),
     "r4q_paged_flash_decode": (i32, [vp, i64, vp, vp, vp, i64, i32, i32, i32, vp, sz_t, vp]),
     "r4q_kernel_status": (i32, [i32]),
+    "r4q_debug_wait_limit": (i64, [i64]),
     "r4q_debug_status_of": (i32, [i32, i32, i32]),
     "r4q_kv_copy_pages": (i32, [vp, i64, i64, i64, i64, i32, vp, vp, i32, vp]),
     "r4q_kv_table_set": (i32, [vp, i64, i32, i32, vp, vp, vp, i32, vp]),
