@@ -20,6 +20,11 @@ __device__ __forceinline__ F2 add(F2 a, F2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
   return F2(d);
 }
+__device__ __forceinline__ F2 sub(F2 a, F2 b) {
+  uint64_t d;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
+  return F2(d);
+}
 __device__ __forceinline__ F2 mul(F2 a, F2 b) {
   uint64_t d;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));

@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, kResident)
   // ---- one pass: chunks of the row, dealt to the warps of the cluster in turn
   constexpr bool kFused = std::is_same<X, __half>::value;    // t in one multiply-add
   const F2 l2e(kLog2e, kLog2e);
-  F2 S2(0.f, 0.f), A2(0.f, 0.f), shift(0.f, 0.f);
+  F2 SA(0.f, 0.f), low(0.f, 0.f), shift(0.f, 0.f);   // S and A, and what their additions rounded away
   float most = -INFINITY, M = 0.f;           // running maximum; what t is relative to: m, or m log2(e) rounded
   float best = -INFINITY;
   int best_w = -1, before = 0, nan = 0;      // best_w: first word of the chunk with the thread's largest value
@@ -403,14 +403,15 @@ __global__ void __launch_bounds__(kThreads, kResident)
     if (c > most) {
       const float to = kFused ? c * kLog2e : c;
       const float d = most == -INFINITY ? kTiny : fmaxf(kFused ? M - to : (M - to) * kLog2e, kTiny), f = ex2(d);
-      A2 = mul(F2(f, f), fma(S2, F2(d, d), A2));
-      S2 = mul(F2(f, f), S2);
+      const float2 a = SA.get(), b = low.get();
+      SA = F2(f * a.x, f * fmaf(a.x, d, a.y));
+      low = F2(f * b.x, f * fmaf(b.x, d, b.y));
       most = c;
       M = to;
       shift = F2(-to, -to);
     }
     // the chunk's sums; -inf gives 0 * -inf in A, and only then t is bounded below
-    F2 Ac(0.f, 0.f);
+    F2 Sc(0.f, 0.f), Ac(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
       float x[n];
@@ -420,11 +421,11 @@ __global__ void __launch_bounds__(kThreads, kResident)
         const F2 two(x[q], x[q + 1]), t = kFused ? fma(two, l2e, shift) : mul(add(two, shift), l2e);
         const float2 f = t.get();
         const F2 e(ex2(f.x), ex2(f.y));
-        S2 = add(S2, e);
+        Sc = add(Sc, e);
         Ac = fma(e, t, Ac);
       }
     }
-    const float2 sum = Ac.get();
+    float2 sum = Ac.get();
     if (sum.x + sum.y != sum.x + sum.y) {
       Ac = F2(0.f, 0.f);
 #pragma unroll 1
@@ -439,8 +440,14 @@ __global__ void __launch_bounds__(kThreads, kResident)
           Ac = fma(F2(ex2(fmaxf(f.x, kTiny)), ex2(fmaxf(f.y, kTiny))), t, Ac);
         }
       }
+      sum = Ac.get();
     }
-    A2 = add(A2, Ac);
+    {   // to the thread's sums, whose rounding errors go along (Kahan 1965): a long row's would add up
+      const float2 s = Sc.get();
+      const F2 y = sub(F2(s.x + s.y, sum.x + sum.y), low), t = add(SA, y);
+      low = sub(sub(t, SA), y);
+      SA = t;
+    }
     if (has_t && (c >= xt || xt != xt)) {    // what precedes the token
       uint32_t th[kUnroll];
       bool has = !plain_t;
@@ -483,10 +490,10 @@ __global__ void __launch_bounds__(kThreads, kResident)
   Sums s;
   s.m = most;
   {
-    const float2 a = S2.get(), b = A2.get();
+    const float2 a = SA.get();
     const float off = kFused && most > -INFINITY && most < INFINITY ? fmaf(most, kLog2e, -M) : 0.f, f = ex2(-off);
-    s.S = (a.x + a.y) * f;
-    s.A = (b.x + b.y - off * (a.x + a.y)) * f;
+    s.S = a.x * f;
+    s.A = (a.y - off * a.x) * f;
   }
 
   // ---- bounds of the largest key of the thread, and the CTA's sums
