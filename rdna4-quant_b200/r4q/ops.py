@@ -412,6 +412,8 @@ def residual_f16(a: torch.Tensor, res: torch.Tensor | None, out: torch.Tensor, s
 # ------------------------------------------------------------- paged KV cache ---
 # The operators from here on check their tensors and allocate in the native
 # module _r4q_torch (csrc/torch_ops.cpp), which calls the library that lib.py loaded.
+# It is bound to one build of torch, so it is loaded when one of them is first
+# called: the others do not depend on it.
 def _load_native():
     path = L._PKG / "_r4q_torch.so"
     if not path.exists():
@@ -426,7 +428,17 @@ def _load_native():
     return mod
 
 
-_native = _load_native()
+class _Native:
+    _lock = threading.Lock()
+
+    def __getattr__(self, name):               # of what is not loaded yet
+        with self._lock:
+            if not self.__dict__:
+                self.__dict__.update({k: f for k, f in vars(_load_native()).items() if not k.startswith("__")})
+        return object.__getattribute__(self, name)
+
+
+_native = _Native()
 
 
 def _checked(r, name: str):
