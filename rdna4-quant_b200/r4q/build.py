@@ -58,6 +58,12 @@ def _torch_command(out: Path) -> list:
             "-Xlinker", f"-rpath,{root / 'lib'}"]
 
 
+def _torch_identity(command) -> str:
+    """What the module is bound to besides its source: the torch and Python builds, and the command."""
+    import torch
+    return "\n".join([torch.__version__, str(torch.version.git_version), sys.version, *command])
+
+
 def build(verbose: bool = False, force: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     headers = list(CSRC.glob("*.cuh")) + list(INCLUDE.glob("*.h"))
@@ -79,13 +85,17 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         return r
 
     module = TORCH_OUT.with_suffix(".so.tmp")
-    stale_module = force or _stale(TORCH_OUT, TORCH_SRC, [INCLUDE / "r4q.h"])
+    command, made_by = _torch_command(module), BUILD / "torch_ops.made_by"
+    about = _torch_identity(command)
+    stale_module = (force or _stale(TORCH_OUT, TORCH_SRC, [INCLUDE / "r4q.h"]) or not made_by.exists()
+                    or made_by.read_text() != about)
     if stale_module:
-        jobs.insert(0, _torch_command(module))      # the longest first
+        jobs.insert(0, command)                     # the longest first
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
         list(ex.map(run, jobs))
     if stale_module:
         os.replace(module, TORCH_OUT)
+        made_by.write_text(about)
         jobs.pop(0)
     if jobs or force or not OUT.exists() or any(o.stat().st_mtime > OUT.stat().st_mtime for o in objs):
         tmp = OUT.with_suffix(".so.tmp")

@@ -68,3 +68,35 @@ def test_threads_that_use_it_first_at_once():
     """
     r = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "served" in r.stdout, r.stderr[-2000:]
+
+
+def test_build_remakes_it_for_another_torch(monkeypatch, tmp_path):
+    """build() with every compiler run recorded instead: nothing to do twice, the module alone after a torch upgrade."""
+    import torch
+    from r4q import build as b
+    src, out = tmp_path / "csrc", tmp_path / "out"
+    src.mkdir(), out.mkdir()
+    (src / "torch_ops.cpp").write_text("")
+    (src / "a.cu").write_text("")
+    for name, value in dict(CSRC=src, TORCH_SRC=src / "torch_ops.cpp", OUT=out / "libr4q.so",
+                            TORCH_OUT=out / "_r4q_torch.so", BUILD=out / "build").items():
+        monkeypatch.setattr(b, name, value)
+    runs = []
+
+    def record(cmd, **kw):
+        made = Path(cmd[cmd.index("-o") + 1])
+        made.write_text("")
+        runs.append(made.name)
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+    monkeypatch.setattr(b.subprocess, "run", record)
+    b.build()
+    assert sorted(runs) == ["_r4q_torch.so.tmp", "a.o", "libr4q.so.tmp"] and (out / "_r4q_torch.so").exists()
+    runs.clear()
+    b.build()
+    assert runs == []
+    monkeypatch.setattr(torch, "__version__", "99.0")
+    b.build()
+    assert runs == ["_r4q_torch.so.tmp"]
+    runs.clear()
+    b.build()
+    assert runs == []
