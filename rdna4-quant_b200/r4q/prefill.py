@@ -63,10 +63,14 @@ def prefill_logits(hidden: torch.Tensor, qkv_w, qkv_s, o_w, o_s, gu_w, gu_s, dow
     cache), so decoding can continue at position M.  With ``pages``
     (r4q.paged.PagedKVCache) they are written to the pages of sequence
     ``batch_row`` instead, which holds M positions already
-    (``pages.extend({batch_row: M})``).  ``last_only`` returns the logits of
+    (``pages.extend({batch_row: M})``), with the scales that belong to them
+    (``PagedKVCache(k_scales=...)``).  ``last_only`` returns the logits of
     the last position only [1, lm_N]."""
-    if pages is not None and k_caches is not None:
-        raise ValueError("prefill_logits: k_caches or pages, not both")
+    if pages is not None:
+        given = [n for n, x in (("k_caches", k_caches), ("v_caches", v_caches), ("k_scales", k_scales),
+                                ("v_scales", v_scales)) if x is not None]
+        if given:
+            raise ValueError(f"prefill_logits: pages bring their own caches and scales, not with {', '.join(given)}")
     x = hidden.reshape(-1, int(hidden_size)).contiguous()
     M, D = x.shape
     dev = x.device

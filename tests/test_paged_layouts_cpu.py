@@ -45,3 +45,11 @@ def test_a_table_cell_twice_is_refused():
     random.Random(1).shuffle(many)
     for cells in ([(0, 0), (0, 0)], [(1, 2), (2, 1), (1, 2)], many + [many[7]]):
         assert put(cells) == -1 and "twice" in L.last_error()
+
+
+@pytest.mark.parametrize("kw", ["k_caches", "v_caches", "k_scales", "v_scales"])
+def test_prefill_into_pages_refuses_what_it_would_ignore(kw):
+    from r4q import paged, prefill
+    pages = paged.PagedKVCache(1, 4, 2, 16, 1, 4, "cpu")
+    with pytest.raises(ValueError, match=kw):
+        prefill.prefill_logits(*[None] * 25, pages=pages, **{kw: [torch.ones(2)]})
