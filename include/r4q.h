@@ -254,10 +254,10 @@ enum { R4Q_KV_FULL_RANGE = 8 };
  * half-split rotation (row pos[m] of the tables, fp16 [tab_rows][tab_stride])
  * to q and k first, in fp32 with one rounding, as r4q_head_norm_rope does;
  * q_out (ldqo) and k_out (ldko; NULL skips) receive them and may alias q, k.
- * The stored bytes are those of r4q_head_norm_rope's KV write.  That codec
- * stores every |x / scale| from 248 on as 448; with R4Q_KV_FULL_RANGE 256 .. 448
- * are stored as E4M3 has them (all readers decode both), for scales that bring
- * the largest values near 448.
+ * Without R4Q_KV_FULL_RANGE the stored bytes are those of r4q_head_norm_rope's KV
+ * write, whose codec stores every |x / scale| from 248 on as 448; with it 256 .. 448
+ * are stored as E4M3 has them (all readers decode both), which scales that bring the
+ * largest values near 448 need (ops.paged_kv_write and PagedKVCache set it).
  * A token with pos[m] < 0 is padding: nothing of it is written.  A row,
  * position, page or table row out of range writes nothing and is reported by
  * r4q_kernel_status.  Two tokens of one call must not name one position.

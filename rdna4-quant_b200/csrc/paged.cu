@@ -25,8 +25,10 @@ __device__ int g_write_status;
 // 32-block: the RoPE partners i, i + 64 and the terms that head_kernel
 // (r4q_head_norm_rope) adds in one lane are in one lane here too, and a butterfly
 // over the half finishes the sum of squares in its order.  Norm and rotation equal
-// that kernel's to the bit, so a paged cache holds the bytes that the contiguous
-// one would.  Bound: issue slots, so the arithmetic is two-wide fp32: 8192 tokens
+// that kernel's to the bit, and K is encoded from fp32 as by its KV write: below 248
+// (and, without R4Q_KV_FULL_RANGE, from there on too) a decode step stores the bytes
+// that it would.  A contiguous prefill rounds K to fp16 first, so that its codes may
+// be a step away from these.  Bound: issue slots, so the arithmetic is two-wide fp32: 8192 tokens
 // of 40/8 heads 60 us, 3.6 TB/s (72 us with scalar fp32 and comparisons per value;
 // a warp per head, 4 bytes a lane, 92).
 constexpr int kPairs = 2;
